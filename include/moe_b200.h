@@ -201,6 +201,31 @@ int moe_nf4_dequant(const uint8_t* packed, const float* code, const float* absma
                     void* out, int64_t n_elems, int dtype_out, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Expert products on 8-bit weights.  No counterpart in the reference, whose quantised weights are 4-bit
+ * (qwen3_moe_fused/grouped_gemm/forward_4bit.py).
+ * Weights: e4m3 codes w (E,N,K) and fp32 scales ws (E, ceil(N/128), ceil(K/128)); a weight is code * scale of its block.
+ * Activations: e4m3 codes q (M,K) and fp32 scales s (ceil(K/128), M): block-major, one power of two for each 128 values of a row,
+ * the smallest with max|x| <= 448 s (at least 2^-100), NaN for a block that holds an infinity or a NaN.  Codes are rounded
+ * to nearest, ties to even.
+ * ------------------------------------------------------------------------------- */
+int moe_fp8_quantize_rows(const void* x, int dtype, int64_t M, int K, void* q, float* s, void* stream);
+
+/* which = 0: y[t,n] = sum_kb s[kb,t] ws[e,n/128,kb] sum_{k in kb} q[t,k] w[e,n,k],  w (E,N,K)
+ * which = 1: y[t,n] = sum_kb s[kb,t] ws[e,kb,n/128] sum_{k in kb} q[t,k] w[e,k,n],  w (E,K,N)   (the gradient of x)
+ * plus the same product of q2, s2, w2, ws2 (NULL: none), in one fp32 accumulator that is rounded once to dtype_out.  Rows
+ * are grouped as in moe_grouped_gemm_fwd; E <= 65535. */
+int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2,
+                         const float* s2, const void* w2, const float* ws2, const void* m_sizes, int m_sizes_dtype, void* y,
+                         int64_t M, int N, int K, int E, int dtype_out, void* stream);
+
+/* h = silu(e) g of fp32 products e, g (M,I), quantised to hq, hs; with keep_e, keep_g (both or neither) e and g are kept in
+ * dtype.  And the gradients of e and g (in dtype, as kept) from the fp32 gradient of h, quantised. */
+int moe_fp8_silu_quantize(const float* e, const float* g, int64_t M, int I, void* hq, float* hs, void* keep_e, void* keep_g,
+                          int dtype, void* stream);
+int moe_fp8_silu_bwd_quantize(const float* dh, const void* e, const void* g, int64_t M, int I, void* deq, float* des, void* dgq,
+                              float* dgs, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * SiLU-mul.  Replaces qwen3_moe_fused/kernels/silu_mul.py:114-161.
  *   fwd:         h = dtype(silu_f32(e)) * g
  *   bwd:         de, dg from dh, e, g
@@ -286,6 +311,28 @@ int moe_lora_mlp_bwd(const moe_lora_weights* w, const moe_lora_grads* grads, con
  * Replaces the autograd of qwen3_moe_fused/modular_qwen3_moe_fused.py:110-115. */
 int moe_combine_bwd(const void* dout, const void* y, const int32_t* inv_sort_idx, const void* weights, void* dy,
                     void* dweights, int64_t T, int k, int H, int dtype, void* stream);
+
+/* The residual stream around a block, with the RMS norm in front of the next one:
+ *   sum[t,:] = residual[t,:] + scale * sum_j weights[t,j] * y[inv_sort_idx[t*k+j],:],   normed = sum / rms(sum) * gamma,
+ * rms(s) = sqrt(mean(s^2) + eps).  inv_sort_idx NULL: y has T rows and is added as it is (weights NULL, k 1).  residual NULL:
+ * zeros.  sum or normed may be NULL (not wanted); gamma is read for normed.  rstd (T fp32, may be NULL): 1 / rms(sum), what the
+ * backward needs.  fp32 in between; sum and normed are each rounded once to dtype.  1 <= H <= 24576.
+ * inv_sort_idx names each of the T*k rows of y once, as moe_sort_by_expert's idx does.
+ * Replaces qwen3_moe_fused/modular_qwen3_moe_fused.py:112-115 together with the addition and the norm that follow it in the
+ * layer. */
+int moe_combine_add_rms_norm(const void* y, const int32_t* inv_sort_idx, const void* weights, const void* residual,
+                             const void* gamma, float scale, float eps, void* sum, void* normed, float* rstd, int64_t T, int k,
+                             int H, int dtype, void* stream);
+
+/* Its gradients from those of normed and sum (dnormed, dsum: either may be NULL = zeros): dresidual (T,H), dy (rows of y),
+ * dweights (T,k), dgamma (H), each NULL where it is not wanted.  sum and rstd as the forward wrote them.  dgamma needs ws of
+ * moe_combine_add_rms_norm_bwd_ws_bytes bytes, 16-byte aligned (scratch), and is the same in every run.
+ * No counterpart in the reference, which leaves this to autograd. */
+size_t moe_combine_add_rms_norm_bwd_ws_bytes(int64_t T, int H);
+int moe_combine_add_rms_norm_bwd(const void* dnormed, const void* dsum, const void* sum, const float* rstd, const void* gamma,
+                                 const void* y, const int32_t* inv_sort_idx, const void* weights, float scale, void* dresidual,
+                                 void* dy, void* dweights, void* dgamma, int64_t T, int k, int H, int dtype, void* ws,
+                                 size_t ws_bytes, void* stream);
 
 /* y = sum_i x_i W_i^T (which = 0, W_i (E, N, K_i)) or sum_i x_i W_i (which = 1, W_i (E, K_i, N)) per expert, the n <= 4
  * operand pairs contracted into one fp32 accumulator and rounded once.  x_i has M rows of K_i elements, ldx[i] apart.

@@ -3,7 +3,7 @@
 // All of them move 16 bytes per thread per access when pointers and extents allow it
 // and fall back to scalar accesses otherwise; grids are a multiple of the SM count and
 // loop with a grid stride.
-#include "common.cuh"
+#include "vec.cuh"
 
 namespace moe {
 
@@ -14,21 +14,6 @@ static inline int ew_grid(int64_t work_items) {
   const int64_t cap = (int64_t)sm_count() * 16;
   int64_t g = want < cap ? want : cap;
   return (int)(g < 1 ? 1 : g);
-}
-
-static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); T v[N]; };
-
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* p) {
-  Vec<T> r;
-  *reinterpret_cast<uint4*>(r.v) = *reinterpret_cast<const uint4*>(p);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
-  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.v);
 }
 
 // Sigmoid in fp32.  fp32 tensors take the IEEE division; 16-bit tensors take the hardware

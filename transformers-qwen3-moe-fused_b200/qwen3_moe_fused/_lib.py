@@ -11,6 +11,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 F32, BF16, F16, I32, I64 = 0, 1, 2, 3, 4
 ERR_UNSUPPORTED = -5  # MOE_ERR_UNSUPPORTED: the selected kernel family does not cover the request
@@ -47,6 +48,10 @@ SIGNATURES = {
     "moe_grouped_gemm_dx_nf4": (_I, [_P, _P, _P, _P, _I, _P, _I, _P, _L, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "moe_nf4_dequant": (_I, [_P, _P, _P, _I, _P, _L, _I, _P]),
     "moe_absmax_unnest": (_I, [_P, _P, _P, _I, _P, _P, _L, _P]),
+    "moe_fp8_quantize_rows": (_I, [_P, _I, _L, _I, _P, _P, _P]),
+    "moe_grouped_gemm_fp8": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _P]),
+    "moe_fp8_silu_quantize": (_I, [_P, _P, _L, _I, _P, _P, _P, _P, _I, _P]),
+    "moe_fp8_silu_bwd_quantize": (_I, [_P, _P, _P, _L, _I, _P, _P, _P, _P, _I, _P]),
     "moe_silu_mul_fwd": (_I, [_P, _P, _P, _L, _I, _P]),
     "moe_silu_mul_bwd": (_I, [_P, _P, _P, _P, _P, _L, _I, _P]),
     "moe_silu_mul_bwd_inplace": (_I, [_P, _P, _P, _L, _I, _P]),
@@ -56,6 +61,9 @@ SIGNATURES = {
     "moe_expand_rows": (_I, [_P, _P, _I, _P, _L, _I, _I, _P]),
     "moe_combine": (_I, [_P, _P, _P, _P, _L, _I, _I, _I, _P]),
     "moe_combine_bwd": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _P]),
+    "moe_combine_add_rms_norm": (_I, [_P, _P, _P, _P, _P, _F, _F, _P, _P, _P, _L, _I, _I, _I, _P]),
+    "moe_combine_add_rms_norm_bwd_ws_bytes": (_Z, [_L, _I]),
+    "moe_combine_add_rms_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _L, _I, _I, _I, _P, _Z, _P]),
     "moe_block_fwd_scratch_bytes": (_Z, [_L, _I, _I, _I, _I, _I]),
     "moe_block_fwd": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "moe_lora_mlp_fwd": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P]),
@@ -169,6 +177,12 @@ def workspace(device: torch.device, nbytes: int) -> tuple[int | None, int]:
         buf = torch.empty(max(nbytes + 128, 1 << 16), device=device, dtype=torch.uint8)
         _WORKSPACES[key] = buf
     return (buf.data_ptr() + 127) & ~127, nbytes
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode derivative.  Grad mode does not switch forward mode off, and a call that
+    takes addresses would lose the tangent without a word: such tensors go through the autograd functions, which raise."""
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors if t is not None)
 
 
 def is_int_tensor(x: torch.Tensor) -> bool:
