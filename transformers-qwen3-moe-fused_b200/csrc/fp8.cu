@@ -1,4 +1,5 @@
-// Expert products on 8-bit weights: quantisation of activations and the products on CUDA cores, for any extents.
+// Expert products on 8-bit weights: quantisation of activations, the products on CUDA cores for any extents, and the C ABI of
+// both these and the tensor-core forms (tc_gemm_fp8.cuh).
 //
 //   y[t, n] = sum_kb s[kb, t] ws[e, n / 128, kb] * sum_{k in block kb} q[t, k] w[e, n, k]        (which = 0)
 //   y[t, n] = sum_kb s[kb, t] ws[e, kb, n / 128] * sum_{k in block kb} q[t, k] w[e, k, n]        (which = 1, the gradient of x)
@@ -9,6 +10,11 @@
 #include "vec.cuh"
 
 namespace moe {
+
+bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E);
+int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2, const float* s2,
+                        const void* w2, const float* ws2, const void* m_sizes, int ms64, void* out, int64_t M, int N, int K, int E,
+                        int dtype_out, cudaStream_t stream);
 
 namespace {
 
@@ -285,6 +291,8 @@ MOE_API int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const
   if (!q || !s || !w || !ws || !m_sizes || !y || (q2 && (!s2 || !w2 || !ws2))) return MOE_ERR_NULL;
   const int ms64 = msd == MOE_I64;
   const int path = moe_get_gemm_path();
+  if (path != MOE_PATH_SIMT && path != MOE_PATH_TC_SINGLE && tc_fp8_eligible(q, w, q2, w2, y, M, N, K, E))
+    return tc_grouped_gemm_fp8(which, q, s, w, ws, q2, s2, w2, ws2, m_sizes, ms64, y, M, N, K, E, dtype_out, stream);
   if (path == MOE_PATH_TC || path == MOE_PATH_TC_SINGLE) return MOE_ERR_UNSUPPORTED;
   const Fp8Pairs ops = {{(const uint8_t*)q, (const uint8_t*)q2}, {s, s2}, {(const uint8_t*)w, (const uint8_t*)w2}, {ws, ws2}, q2 ? 2 : 1};
   const dim3 grid((N + S_TILE - 1) / S_TILE, E, S_WORKERS);

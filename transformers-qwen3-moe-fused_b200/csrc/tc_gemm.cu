@@ -587,6 +587,7 @@ tc_fwd_nf4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
 #include "tc_gemm_pair.cuh"
 #include "tc_gemm_dw.cuh"
 #include "tc_gemm_nf4.cuh"
+#include "tc_gemm_fp8.cuh"
 
 namespace moe {
 namespace tc {
@@ -628,6 +629,24 @@ static int make_map(CUtensorMap* map, int dtype, const void* base, uint64_t d0, 
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     snprintf(g_detail, sizeof(g_detail), "cuTensorMapEncodeTiled -> %d: base=%p dims=(%llu,%llu,%llu) box=(64,%u,1) rank=%u",
+             (int)r, base, (unsigned long long)d0, (unsigned long long)d1, (unsigned long long)d2, b1, rank);
+  return r == CUDA_SUCCESS ? MOE_OK : MOE_ERR_UNSUPPORTED;
+}
+
+// Tensor map over 8-bit codes, box = (128 bytes, b1 rows, 1), swizzled like make_map's.
+static int make_map_codes(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t b1) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return MOE_ERR_DEVICE;
+  const cuuint32_t rank = d2 ? 3 : 2;
+  cuuint64_t dims[3] = {d0, d1, d2 ? d2 : 1};
+  cuuint64_t strides[2] = {d0, d0 * d1};
+  cuuint32_t box[3] = {128, b1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    snprintf(g_detail, sizeof(g_detail), "cuTensorMapEncodeTiled -> %d: base=%p dims=(%llu,%llu,%llu) box=(128,%u,1) rank=%u",
              (int)r, base, (unsigned long long)d0, (unsigned long long)d1, (unsigned long long)d2, b1, rank);
   return r == CUDA_SUCCESS ? MOE_OK : MOE_ERR_UNSUPPORTED;
 }
@@ -1217,6 +1236,53 @@ int tc_grouped_gemm_nf4(const void* x, const uint8_t* packed, const float* code,
   } else {
     if ((st = set_smem(tc_fwd_nf4_kernel<false>, bytes)) != MOE_OK) return st;
     tc_fwd_nf4_kernel<false><<<grid, NF4_THREADS, bytes, stream>>>(ma, mq, p, q);
+  }
+  return launch_status();
+}
+
+// What the 8-bit CTA-pair kernel takes: rows of 16-byte multiples on aligned bases, tables of the groups in shared memory.
+bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E) {
+  const uintptr_t bits = (uintptr_t)q | (uintptr_t)w | (uintptr_t)q2 | (uintptr_t)w2 | (uintptr_t)out;
+  if ((bits & 15) || N % 16 || K % 16 || E > tc::MAX_E || M < 1 || M > 0x7fffffffLL - 1024) return false;
+  return pair_tiles_bound(M, E, (N + 255) / 256) < (int64_t)1 << 30;  // tile ids and grids are 32-bit
+}
+
+int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2, const float* s2,
+                        const void* w2, const float* ws2, const void* m_sizes, int ms64, void* out, int64_t M, int N, int K, int E,
+                        int dtype_out, cudaStream_t stream) {
+  using namespace tc;
+  bind_context_once();
+  Fp8Maps maps;
+  memset(&maps, 0, sizeof(maps));
+  Fp8Params p = {};
+  p.m_sizes = m_sizes; p.ms64 = ms64; p.M = M; p.N = N; p.E = E; p.out = out; p.dtype_out = dtype_out;
+  p.kb = (K + F8_BK - 1) / F8_BK;
+  p.n_seg = q2 ? 2 : 1;
+  p.s[0] = s; p.s[1] = s2; p.ws[0] = ws; p.ws[1] = ws2;
+  const int nb = (N + 127) / 128;
+  p.ws_e = (int64_t)nb * p.kb;
+  p.ws_n = which == 0 ? p.kb : 1;
+  p.ws_k = which == 0 ? 1 : nb;
+  p.idesc = make_idesc(0, which, 0, 256, 0);  // format 0: e4m3; the N field is filled per tile
+  int st;
+  for (int i = 0; i < p.n_seg; ++i) {
+    const void* wi = i ? w2 : w;
+    const void* qi = i ? q2 : q;
+    st = which == 0 ? make_map_codes(&maps.w[i], wi, (uint64_t)K, (uint64_t)N, (uint64_t)E, 128)
+                    : make_map_codes(&maps.w[i], wi, (uint64_t)N, (uint64_t)K, (uint64_t)E, F8_BK);
+    if (st != MOE_OK) return st;
+    if ((st = make_map_codes(&maps.x[i], qi, (uint64_t)K, (uint64_t)M, 0, 128)) != MOE_OK) return st;
+    if ((st = make_map_codes(&maps.xs[i], qi, (uint64_t)K, (uint64_t)M, 0, PAIR_SMALL_BOX)) != MOE_OK) return st;
+  }
+  if (dtype_out != MOE_F32 && (st = make_map(&maps.out, dtype_out, out, (uint64_t)N, (uint64_t)M, 0, 32)) != MOE_OK) return st;
+  const int bytes = fp8_smem_bytes(E);
+  const unsigned grid = (unsigned)(2 * pair_tiles_bound(M, E, (N + 255) / 256));
+  if (which == 0) {
+    if ((st = set_smem(pair_fp8_kernel<false>, bytes)) != MOE_OK) return st;
+    pair_fp8_kernel<false><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
+  } else {
+    if ((st = set_smem(pair_fp8_kernel<true>, bytes)) != MOE_OK) return st;
+    pair_fp8_kernel<true><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
   }
   return launch_status();
 }

@@ -250,9 +250,9 @@ __device__ __forceinline__ void pair_store_tile_gate_up(uint8_t* staging, uint32
 //             MMAs to issue); readers: both producers, the MMA thread, 8 epilogue warps.  It runs up
 //             to SCHED_DEPTH tiles ahead, so the round trip of its request is never waited for.
 //   NCTA = 1: the producer thread draws for itself (dW); readers: the MMA thread, 4 epilogue warps.
-template <int NCTA>
+template <int NCTA, int NREADERS = NCTA == 2 ? 11 : 5>
 struct TileFeed {
-  static constexpr int READERS = NCTA == 2 ? 11 : 5;
+  static constexpr int READERS = NREADERS;
   static constexpr uint32_t HOME = NCTA == 2 ? 1 : 0;  // CTA of the drawing thread
   SchedRing* ring;
   uint32_t home_empty0;  // address of the home CTA's empty[0] (shared::cluster window when NCTA = 2)
