@@ -204,7 +204,8 @@ int moe_nf4_dequant(const uint8_t* packed, const float* code, const float* absma
  * Expert products on 8-bit weights.  No counterpart in the reference, whose quantised weights are 4-bit
  * (qwen3_moe_fused/grouped_gemm/forward_4bit.py).
  * Weights: e4m3 codes w (E,N,K) and fp32 scales ws (E, ceil(N/128), ceil(K/128)); a weight is code * scale of its block.
- * Activations: e4m3 codes q (M,K) and fp32 scales s (ceil(K/128), M): block-major, one power of two for each 128 values of a row,
+ * Activations: e4m3 codes q (M,K) and fp32 scales s (ceil(K/128), M): block-major, M rounded up to a multiple of 4 elements
+ * from one block to the next (what lies between is not read or written), one power of two for each 128 values of a row,
  * the smallest with max|x| <= 448 s (at least 2^-100), NaN for a block that holds an infinity or a NaN.  Codes are rounded
  * to nearest, ties to even.
  * ------------------------------------------------------------------------------- */
@@ -217,6 +218,14 @@ int moe_fp8_quantize_rows(const void* x, int dtype, int64_t M, int K, void* q, f
 int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2,
                          const float* s2, const void* w2, const float* ws2, const void* m_sizes, int m_sizes_dtype, void* y,
                          int64_t M, int N, int K, int E, int dtype_out, void* stream);
+
+/* The gated half of the expert MLP in one kernel: e = q w_gate^T, g = q w_up^T (as above, fp32), h = silu(e) g quantised to codes
+ * hq (M,I) and scales hs; with keep_e, keep_g (both or neither, 16-byte aligned) e and g are kept in dtype.  16-bit dtypes,
+ * I and K multiples of 16, 16-byte aligned bases, E <= 1024; MOE_ERR_UNSUPPORTED otherwise (moe_grouped_gemm_fp8 twice and
+ * moe_fp8_silu_quantize give the same up to fp32 sums). */
+int moe_gate_up_silu_fp8(const void* q, const float* s, const void* w_gate, const float* ws_gate, const void* w_up,
+                         const float* ws_up, const void* m_sizes, int m_sizes_dtype, void* hq, float* hs, void* keep_e,
+                         void* keep_g, int64_t M, int I, int K, int E, int dtype, void* stream);
 
 /* h = silu(e) g of fp32 products e, g (M,I), quantised to hq, hs; with keep_e, keep_g (both or neither) e and g are kept in
  * dtype.  And the gradients of e and g (in dtype, as kept) from the fp32 gradient of h, quantised. */

@@ -56,6 +56,9 @@ inline int sm_count() {
   return cached[dev];
 }
 
+// Elements between the blocks of the scales of M quantised rows: whole 16-byte units, as the copy engine wants them.
+inline int64_t fp8_scale_pitch(int64_t M) { return (M + 3) & ~(int64_t)3; }
+
 // moe_grouped_gemm_sum whose product i counts 2^log2_scale[i] times (null: once; at most 2^15 between any two), and
 // moe_grouped_gemm_dw_strided whose gradients are multiplied by alpha / alpha2 ahead of their rounding (gemm_api.cu).
 int grouped_gemm_sum_scaled(int which, int n, const void* const* x, const int64_t* ldx, const void* const* w, const int* K,

@@ -4,17 +4,22 @@
 //   y[t, n] = sum_kb s[kb, t] ws[e, n / 128, kb] * sum_{k in block kb} q[t, k] w[e, n, k]        (which = 0)
 //   y[t, n] = sum_kb s[kb, t] ws[e, kb, n / 128] * sum_{k in block kb} q[t, k] w[e, k, n]        (which = 1, the gradient of x)
 //
-// with q, s from fp8.cuh.  Scales of activations are stored block by block, (ceil(K / 128), M): the scales that a tile of
-// tokens needs for one block of the contraction are consecutive.
+// with q, s from fp8.cuh.  Scales of activations are stored block by block, (ceil(K / 128), M) with rows padded to a
+// multiple of 4: the scales that a tile of tokens needs for one block of the contraction are consecutive.
 #include "fp8.cuh"
 #include "vec.cuh"
 
 namespace moe {
 
-bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E);
+bool tc_fp8_eligible(const void* q, const float* s, const void* w, const void* q2, const float* s2, const void* w2, const void* out,
+                     int64_t M, int N, int K, int E);
 int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2, const float* s2,
                         const void* w2, const float* ws2, const void* m_sizes, int ms64, void* out, int64_t M, int N, int K, int E,
                         int dtype_out, cudaStream_t stream);
+
+int tc_gate_up_silu_fp8(const void* q, const float* s, const void* w_gate, const float* ws_gate, const void* w_up,
+                        const float* ws_up, const void* m_sizes, int ms64, void* hq, float* hs, void* keep_e, void* keep_g,
+                        int64_t M, int I, int K, int E, int dtype, cudaStream_t stream);
 
 namespace {
 
@@ -80,10 +85,11 @@ __device__ __forceinline__ void for_row_blocks(int64_t M, int K, Body body) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 quantize_rows_kernel(const T* __restrict__ x, int64_t M, int K, uint8_t* __restrict__ q, float* __restrict__ scale) {
+  const int64_t pitch = (M + 3) & ~(int64_t)3;
   for_row_blocks(M, K, [&](int64_t row, int col, int kb) {
     float v[8];
     load8<T, VEC>(x + row * K, col, K, v);
-    store_codes<VEC>(v, q + row * K, col, K, scale + (int64_t)kb * M + row);
+    store_codes<VEC>(v, q + row * K, col, K, scale + kb * pitch + row);
   });
 }
 
@@ -92,6 +98,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 silu_quantize_kernel(const float* __restrict__ e, const float* __restrict__ g, int64_t M, int I, uint8_t* __restrict__ hq,
                      float* __restrict__ hs, T* __restrict__ keep_e, T* __restrict__ keep_g) {
+  const int64_t pitch = (M + 3) & ~(int64_t)3;
   for_row_blocks(M, I, [&](int64_t row, int col, int kb) {
     float ve[8], vg[8], h[8];
     load8<float, VEC>(e + row * I, col, I, ve);
@@ -104,7 +111,7 @@ silu_quantize_kernel(const float* __restrict__ e, const float* __restrict__ g, i
         keep_g[row * I + col + i] = from_f32<T>(vg[i]);
       }
     }
-    store_codes<VEC>(h, hq + row * I, col, I, hs + (int64_t)kb * M + row);
+    store_codes<VEC>(h, hq + row * I, col, I, hs + kb * pitch + row);
   });
 }
 
@@ -113,6 +120,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 silu_bwd_quantize_kernel(const float* __restrict__ dh, const T* __restrict__ e, const T* __restrict__ g, int64_t M, int I,
                          uint8_t* __restrict__ deq, float* __restrict__ des, uint8_t* __restrict__ dgq, float* __restrict__ dgs) {
+  const int64_t pitch = (M + 3) & ~(int64_t)3;
   for_row_blocks(M, I, [&](int64_t row, int col, int kb) {
     float vd[8], ve[8], vg[8];
     load8<float, VEC>(dh + row * I, col, I, vd);
@@ -120,8 +128,8 @@ silu_bwd_quantize_kernel(const float* __restrict__ dh, const T* __restrict__ e, 
     load8<T, VEC>(g + row * I, col, I, vg);
 #pragma unroll
     for (int i = 0; i < 8; ++i) gated_silu_bwd(vd[i], ve[i], vg[i], ve[i], vg[i]);
-    store_codes<VEC>(ve, deq + row * I, col, I, des + (int64_t)kb * M + row);
-    store_codes<VEC>(vg, dgq + row * I, col, I, dgs + (int64_t)kb * M + row);
+    store_codes<VEC>(ve, deq + row * I, col, I, des + kb * pitch + row);
+    store_codes<VEC>(vg, dgq + row * I, col, I, dgs + kb * pitch + row);
   });
 }
 
@@ -202,7 +210,7 @@ simt_gemm_fp8_kernel(const Fp8Pairs ops, const void* m_sizes, int ms64, T* __res
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int64_t t = t0 + ty * 4 + u;
-          const float sx = t < row_end ? ops.s[i][(int64_t)kb * M + t] * sw : 0.f;
+          const float sx = t < row_end ? ops.s[i][kb * ((M + 3) & ~(int64_t)3) + t] * sw : 0.f;
 #pragma unroll
           for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(part[u][v], sx, acc[u][v]);
         }
@@ -281,6 +289,21 @@ MOE_API int moe_fp8_silu_bwd_quantize(const float* dh, const void* e, const void
   return launch_status();
 }
 
+MOE_API int moe_gate_up_silu_fp8(const void* q, const float* s, const void* w_gate, const float* ws_gate, const void* w_up,
+                                 const float* ws_up, const void* m_sizes, int msd, void* hq, float* hs, void* keep_e,
+                                 void* keep_g, int64_t M, int I, int K, int E, int dtype, void* stream) {
+  if (!is_float_dtype(dtype) || !is_int_dtype(msd)) return MOE_ERR_DTYPE;
+  if (M < 0 || M > 0x7fffffffLL - 1024 || I < 1 || K < 1 || E < 1) return MOE_ERR_SHAPE;
+  if (M == 0) return MOE_OK;
+  if (!q || !s || !w_gate || !ws_gate || !w_up || !ws_up || !m_sizes || !hq || !hs || !keep_e != !keep_g) return MOE_ERR_NULL;
+  const int path = moe_get_gemm_path();
+  if (path == MOE_PATH_SIMT || path == MOE_PATH_TC_SINGLE || dtype == MOE_F32 || !aligned16(keep_e) || !aligned16(keep_g) ||
+      !tc_fp8_eligible(q, s, w_gate, nullptr, nullptr, w_up, hq, M, I, K, E))
+    return MOE_ERR_UNSUPPORTED;
+  return tc_gate_up_silu_fp8(q, s, w_gate, ws_gate, w_up, ws_up, m_sizes, msd == MOE_I64, hq, hs, keep_e, keep_g, M, I, K, E, dtype,
+                             (cudaStream_t)stream);
+}
+
 MOE_API int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2,
                                  const float* s2, const void* w2, const float* ws2, const void* m_sizes, int msd, void* y,
                                  int64_t M, int N, int K, int E, int dtype_out, void* stream_) {
@@ -291,7 +314,7 @@ MOE_API int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const
   if (!q || !s || !w || !ws || !m_sizes || !y || (q2 && (!s2 || !w2 || !ws2))) return MOE_ERR_NULL;
   const int ms64 = msd == MOE_I64;
   const int path = moe_get_gemm_path();
-  if (path != MOE_PATH_SIMT && path != MOE_PATH_TC_SINGLE && tc_fp8_eligible(q, w, q2, w2, y, M, N, K, E))
+  if (path != MOE_PATH_SIMT && path != MOE_PATH_TC_SINGLE && tc_fp8_eligible(q, s, w, q2, s2, w2, y, M, N, K, E))
     return tc_grouped_gemm_fp8(which, q, s, w, ws, q2, s2, w2, ws2, m_sizes, ms64, y, M, N, K, E, dtype_out, stream);
   if (path == MOE_PATH_TC || path == MOE_PATH_TC_SINGLE) return MOE_ERR_UNSUPPORTED;
   const Fp8Pairs ops = {{(const uint8_t*)q, (const uint8_t*)q2}, {s, s2}, {(const uint8_t*)w, (const uint8_t*)w2}, {ws, ws2}, q2 ? 2 : 1};

@@ -18,6 +18,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "fp8.cuh"
 #include "tc_common.cuh"
 
 namespace moe {
@@ -1241,8 +1242,9 @@ int tc_grouped_gemm_nf4(const void* x, const uint8_t* packed, const float* code,
 }
 
 // What the 8-bit CTA-pair kernel takes: rows of 16-byte multiples on aligned bases, tables of the groups in shared memory.
-bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E) {
-  const uintptr_t bits = (uintptr_t)q | (uintptr_t)w | (uintptr_t)q2 | (uintptr_t)w2 | (uintptr_t)out;
+bool tc_fp8_eligible(const void* q, const float* s, const void* w, const void* q2, const float* s2, const void* w2, const void* out,
+                     int64_t M, int N, int K, int E) {
+  const uintptr_t bits = (uintptr_t)q | (uintptr_t)w | (uintptr_t)q2 | (uintptr_t)w2 | (uintptr_t)out | (uintptr_t)s | (uintptr_t)s2;
   if ((bits & 15) || N % 16 || K % 16 || E > tc::MAX_E || M < 1 || M > 0x7fffffffLL - 1024) return false;
   return pair_tiles_bound(M, E, (N + 255) / 256) < (int64_t)1 << 30;  // tile ids and grids are 32-bit
 }
@@ -1258,12 +1260,13 @@ int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w,
   p.m_sizes = m_sizes; p.ms64 = ms64; p.M = M; p.N = N; p.E = E; p.out = out; p.dtype_out = dtype_out;
   p.kb = (K + F8_BK - 1) / F8_BK;
   p.n_seg = q2 ? 2 : 1;
-  p.s[0] = s; p.s[1] = s2; p.ws[0] = ws; p.ws[1] = ws2;
+  p.s[0] = s; p.s[1] = s2 ? s2 : s; p.ws[0] = ws; p.ws[1] = ws2 ? ws2 : ws;
+  p.pitch = fp8_scale_pitch(M);
   const int nb = (N + 127) / 128;
   p.ws_e = (int64_t)nb * p.kb;
   p.ws_n = which == 0 ? p.kb : 1;
   p.ws_k = which == 0 ? 1 : nb;
-  p.idesc = make_idesc(0, which, 0, 256, 0);  // format 0: e4m3; the N field is filled per tile
+  p.idesc = make_idesc(0, 0, which, 256, 0);  // format 0: e4m3; the N field is filled per tile
   int st;
   for (int i = 0; i < p.n_seg; ++i) {
     const void* wi = i ? w2 : w;
@@ -1275,15 +1278,47 @@ int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w,
     if ((st = make_map_codes(&maps.xs[i], qi, (uint64_t)K, (uint64_t)M, 0, PAIR_SMALL_BOX)) != MOE_OK) return st;
   }
   if (dtype_out != MOE_F32 && (st = make_map(&maps.out, dtype_out, out, (uint64_t)N, (uint64_t)M, 0, 32)) != MOE_OK) return st;
-  const int bytes = fp8_smem_bytes(E);
+  p.stages = fp8_stages(E);
+  const int bytes = fp8_smem_bytes(p.stages, E);
   const unsigned grid = (unsigned)(2 * pair_tiles_bound(M, E, (N + 255) / 256));
   if (which == 0) {
-    if ((st = set_smem(pair_fp8_kernel<false>, bytes)) != MOE_OK) return st;
-    pair_fp8_kernel<false><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
+    if ((st = set_smem(pair_fp8_kernel<false, false>, bytes)) != MOE_OK) return st;
+    pair_fp8_kernel<false, false><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
   } else {
-    if ((st = set_smem(pair_fp8_kernel<true>, bytes)) != MOE_OK) return st;
-    pair_fp8_kernel<true><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
+    if ((st = set_smem(pair_fp8_kernel<true, false>, bytes)) != MOE_OK) return st;
+    pair_fp8_kernel<true, false><<<grid, F8_THREADS, bytes, stream>>>(maps, p);
   }
+  return launch_status();
+}
+
+// h = silu(q wg^T) * (q wu^T) as codes and scales, and with keep_e, keep_g the projections in dtype.
+int tc_gate_up_silu_fp8(const void* q, const float* s, const void* w_gate, const float* ws_gate, const void* w_up,
+                        const float* ws_up, const void* m_sizes, int ms64, void* hq, float* hs, void* keep_e, void* keep_g,
+                        int64_t M, int I, int K, int E, int dtype, cudaStream_t stream) {
+  using namespace tc;
+  bind_context_once();
+  Fp8Maps maps;
+  memset(&maps, 0, sizeof(maps));
+  Fp8Params p = {};
+  p.m_sizes = m_sizes; p.ms64 = ms64; p.M = M; p.N = I; p.E = E; p.dtype_out = dtype;
+  p.out = hq; p.out_s = hs; p.keep_e = keep_e; p.keep_g = keep_g;
+  p.kb = (K + F8_BK - 1) / F8_BK;
+  p.n_seg = 1;
+  p.s[0] = p.s[1] = s; p.ws[0] = ws_gate; p.ws[1] = ws_up;
+  p.pitch = fp8_scale_pitch(M);
+  p.ws_e = (int64_t)((I + 127) / 128) * p.kb;
+  p.ws_n = p.kb;
+  p.ws_k = 1;
+  p.idesc = make_idesc(0, 0, 0, 256, 0);
+  int st;
+  if ((st = make_map_codes(&maps.w[0], w_gate, (uint64_t)K, (uint64_t)I, (uint64_t)E, 64)) != MOE_OK) return st;
+  if ((st = make_map_codes(&maps.w[1], w_up, (uint64_t)K, (uint64_t)I, (uint64_t)E, 64)) != MOE_OK) return st;
+  if ((st = make_map_codes(&maps.x[0], q, (uint64_t)K, (uint64_t)M, 0, 128)) != MOE_OK) return st;
+  if ((st = make_map_codes(&maps.xs[0], q, (uint64_t)K, (uint64_t)M, 0, PAIR_SMALL_BOX)) != MOE_OK) return st;
+  p.stages = fp8_stages(E);
+  const int bytes = fp8_smem_bytes(p.stages, E);
+  if ((st = set_smem(pair_fp8_kernel<false, true>, bytes)) != MOE_OK) return st;
+  pair_fp8_kernel<false, true><<<(unsigned)(2 * pair_tiles_bound(M, E, (I + 127) / 128)), F8_THREADS, bytes, stream>>>(maps, p);
   return launch_status();
 }
 

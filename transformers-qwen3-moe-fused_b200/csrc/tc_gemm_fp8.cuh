@@ -4,38 +4,37 @@
 //   pair_fp8_kernel<true> : y[t,n] = sum_kb s[kb,t] ws[e,kb,n/128] sum_{k in kb} q[t,k] w[e,k,n]     A = w MN-major
 // over one or two operand pairs of the same contraction length into one result.
 //
-// Tiling as in pair_fwd_kernel: accumulator rows are 256 weight rows (128 per CTA, one scale block each), accumulator columns
-// up to 256 tokens.  The scales are arbitrary fp32 numbers, so the tensor cores cannot apply them: every block of 128 of the
+// Accumulator rows are up to 256 tokens (128 per CTA), columns up to 256 weight rows, the other way round than in
+// pair_fwd_kernel.  The scales are arbitrary fp32 numbers, so the tensor cores cannot apply them: every block of 128 of the
 // contraction (one stage: 128 rows x 128 bytes of either operand in each CTA) is a sum of its own in TMEM, and 8 epilogue
-// warps add it to fp32 sums in registers with its factor, acc += s ws * block.  Two accumulators of 256 columns alternate, so
-// the addition of one block runs beside the MMAs of the next: 512 cycles of MMA for a full tile, against 64 packed FMAs, 8 TMEM
-// loads and 8 shared-memory loads for each of the 8 warps.
+// warps add it to fp32 sums in registers with its factor, acc += s ws * block.  A thread owns one token and 128 columns, one
+// block of weight rows: its factor is one number for all of them, and nothing crosses threads.  Two accumulators of 256
+// columns alternate, so the addition of one block runs beside the MMAs of the next: 512 cycles of MMA, 256 of TMEM loads,
+// 285 of packed FMAs on each quarter of the SM.
+// (With weight rows as accumulator rows the factor changes from column to column: in the fragment shape 16x256b, where a thread
+// needs few of them, TMEM loads run at half the rate (535 cycles for 256 columns, measured, against 260 in the shape
+// 32x32b), and forward / dX at 65536 rows, 2048 -> 1536, took 401 / 424 us.)
 //
-// In the accumulator-fragment shape (16x256b) a thread holds 2 of every 8 columns and 4 of the warp's 32 rows: a factor is
-// loaded once for 4 values, and two loads of 16 bytes bring the factors of 32 columns (they are stored in that order by the
-// warp that multiplies s with ws, `scale_pos`).  A warp owns 32 accumulator rows and every other run of 32 columns: 128 sums
-// in each thread, hence the register split (8 epilogue warps 208, the 4 others 88).
-//
-// A group of r rows is cut into ceil(r / 256) tiles of about equal width (a multiple of 32): the MMAs' cost goes with the columns, the
-// weight stream with the number of tiles.
+// The price is that a tile costs 256 rows of MMAs whatever it holds; groups of few rows are bound by their weights, and warps
+// without rows skip the additions.
 #pragma once
 
 namespace moe {
 namespace tc {
 
-constexpr int F8_THREADS = 384;        // TMA, MMA, scales, one idle warp; 8 epilogue warps
+constexpr int F8_THREADS = 384;        // TMA, MMA, tiles, one idle warp; 8 epilogue warps
 constexpr int F8_BK = 128;             // contraction values (bytes) of a stage
 constexpr int F8_UMMA_K = 32;
 constexpr int F8_HALF_BYTES = 128 * F8_BK;
 constexpr int F8_STAGE_BYTES = 2 * F8_HALF_BYTES;
 constexpr int F8_STAGES = 5;
-constexpr int F8_SLOTS = 8;            // blocks of factors in flight
-constexpr int F8_READERS = 21;         // of the tile ring: 2 producers, 2 scale warps, the MMA thread, 16 epilogue warps
+constexpr int F8_READERS = 5;          // of the pair's tile ring: 2 producers, 2 tile warps, the MMA thread
+constexpr int F8_TILES = 2;            // decoded tiles on their way to the epilogue warps
 constexpr int F8_EPI_REGS = 208, F8_OTHER_REGS = 88;
 static_assert(256 * F8_EPI_REGS + 128 * F8_OTHER_REGS <= F8_THREADS * 168, "shares of the registers that the CTA is launched with");
 
 struct Fp8Maps {
-  CUtensorMap w[2];   // weights
+  CUtensorMap w[2];   // weights (GATE_UP: gate, up)
   CUtensorMap x[2];   // codes of the activations, boxes of 128 rows
   CUtensorMap xs[2];  // the same in boxes of PAIR_SMALL_BOX rows
   CUtensorMap out;    // 16-bit outputs, boxes of 32 rows x 64
@@ -46,13 +45,18 @@ struct Fp8Params {
   int ms64;
   int64_t M;
   int N, E;
+  int stages;
   int kb;               // blocks of the contraction
   int n_seg;            // operand pairs
+  int64_t pitch;        // of s
   const float* s[2];    // (kb, M)
   const float* ws[2];
   int64_t ws_e;         // strides of a weight scale: expert, block of rows, block of the contraction
   int ws_n, ws_k;
-  void* out;
+  void* out;            // GATE_UP: codes of h
+  float* out_s;         // GATE_UP: scales of h
+  void* keep_e;         // GATE_UP: the projections in dtype_out, or null
+  void* keep_g;
   int dtype_out;
   uint32_t idesc;
 };
@@ -62,39 +66,48 @@ struct Fp8Control {
   uint64_t empty[F8_STAGES];
   uint64_t tmem_full[2];
   uint64_t tmem_free[2];   // 16 warps; the leader CTA's copies are the ones used
-  uint64_t sfull[F8_SLOTS];
-  uint64_t sempty[F8_SLOTS];
+  uint64_t tile_full[F8_TILES];   // the tile warp
+  uint64_t tile_empty[F8_TILES];  // 8 epilogue warps
   SchedRing sched;
   uint64_t cancel_bar;
   alignas(16) uint4 cancel_response;
+  int4 tiles[F8_TILES];           // expert (-1: no more tiles), first token, first column, first row past the expert
   uint32_t tmem_base;
   int abort_flag;
 };
 
-enum Fp8WaitCode { FW_SFULL = 24, FW_SEMPTY = 25 };
+enum Fp8WaitCode { FW_TILE_FULL = 24, FW_TILE_EMPTY = 25 };
 
-constexpr int F8_STAGING_BYTES = 2 * 2 * 2 * PAIR_STAGING_BYTES;  // 2 warpgroups x 2 buffers x 2 halves of the weight rows
-static int fp8_smem_bytes(int E) {
-  return F8_STAGES * F8_STAGE_BYTES + F8_STAGING_BYTES + F8_SLOTS * 1024 + (int)sizeof(Fp8Control) + 2 * (E + 1) * 4 + 1024;
+constexpr int F8_ROWS = 256;                       // tokens of a tile
+constexpr int F8_WARP_STAGING = 32 * 128;          // 32 tokens x 64 columns x 16 bit, two of them for each epilogue warp
+constexpr int F8_STAGING_BYTES = 8 * 2 * F8_WARP_STAGING;
+static int fp8_smem_bytes(int stages, int E) {
+  return stages * F8_STAGE_BYTES + F8_STAGING_BYTES + (int)sizeof(Fp8Control) + 2 * (E + 1) * 4 + 1024;
 }
-
-// Where the factor of column `col` of a run of 32 lies: thread t of a warp needs those of columns 8g + 2(t%4) and +1.
-__device__ __forceinline__ int scale_pos(int col) { return ((col >> 1) & 3) * 8 + (col >> 3) * 2 + (col & 1); }
+// Deepest ring that fits (tables of up to 1024 experts leave room for four stages).
+static int fp8_stages(int E) { return fp8_smem_bytes(F8_STAGES, E) <= SMEM_LIMIT ? F8_STAGES : F8_STAGES - 1; }
 
 struct Fp8Tile {
-  int e, t0, n0, n_main, t_end;
+  int e, t0, n0;
+  int n;      // columns of the MMA, a multiple of 32
+  int t_end;  // first row past the expert
 };
 
-template <bool W_MN>
+// W_MN: the weight is (E, K, N), read MN-major (the gradient of x).
+// GATE_UP: 128 features of two weights (E, I, K): columns [gate f..f+63][up f..f+63] from the leader's half of the B operand,
+// the next 64 features from the other CTA's, so a thread holds gate and up of the same 64 features of its token.  The epilogue
+// writes h = silu(gate) * up as codes and scales (the scale's 128 features are those of two threads of one CTA), and the
+// projections themselves in 16 bits where a backward pass wants them.
+template <bool W_MN, bool GATE_UP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(F8_THREADS, 1)
 pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
-  constexpr int TILE_N = 256;
+  static_assert(!(W_MN && GATE_UP), "gate and up read K-major weights");
+  constexpr int TILE_N = GATE_UP ? 128 : 256;  // output columns of a tile
   constexpr uint32_t TMEM_COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* staging = smem + F8_STAGES * F8_STAGE_BYTES;
-  float* factors = reinterpret_cast<float*>(staging + F8_STAGING_BYTES);
-  Fp8Control* ctl = reinterpret_cast<Fp8Control*>(factors + F8_SLOTS * 256);
+  uint8_t* staging = smem + p.stages * F8_STAGE_BYTES;
+  Fp8Control* ctl = reinterpret_cast<Fp8Control*>(staging + F8_STAGING_BYTES);
   int* row_start = reinterpret_cast<int*>(ctl + 1);
   int* tt_start = row_start + (p.E + 1);
   volatile int* abort_flag = &ctl->abort_flag;
@@ -105,9 +118,9 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < F8_STAGES; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
+    for (int s = 0; s < p.stages; ++s) { mbar_init(&ctl->full[s], 1); mbar_init(&ctl->empty[s], 1); }
     for (int a = 0; a < 2; ++a) { mbar_init(&ctl->tmem_full[a], 1); mbar_init(&ctl->tmem_free[a], 16); }
-    for (int q = 0; q < F8_SLOTS; ++q) { mbar_init(&ctl->sfull[q], 32); mbar_init(&ctl->sempty[q], 8); }
+    for (int q = 0; q < F8_TILES; ++q) { mbar_init(&ctl->tile_full[q], 1); mbar_init(&ctl->tile_empty[q], 8); }
     Feed::init(&ctl->sched);
     mbar_init(&ctl->cancel_bar, 1);
     ctl->abort_flag = 0;
@@ -119,7 +132,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
     tmem_alloc_pair(&ctl->tmem_base, TMEM_COLS);
     tmem_relinquish_pair();
   }
-  build_group_tables(p.m_sizes, p.ms64, p.E, p.M, PAIR_TOKENS, row_start, tt_start);
+  build_group_tables(p.m_sizes, p.ms64, p.E, p.M, F8_ROWS, row_start, tt_start);
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
@@ -129,25 +142,18 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
   const int64_t total_tiles = (int64_t)tt_start[p.E] * n_tiles;
   const int steps = p.kb * p.n_seg;  // stages of a tile
 
+  // Within an expert the token tile varies fastest: neighbouring tiles read the same weight slice.
   auto decode = [&](int tile) {
     Fp8Tile t;
     const int q = tile / n_tiles;
     t.e = find_group(tt_start, p.E, q);
     const int tt_e = tt_start[t.e + 1] - tt_start[t.e];
     const int j = tile - tt_start[t.e] * n_tiles;
-    const int jt = j % tt_e;
-    t.t_end = row_start[t.e + 1];
-    const int rows = t.t_end - row_start[t.e];
-    // (several tiles: whole runs of 32 columns, and every tile has rows, since 256 (tiles - 1) < rows)
-    const int width = tt_e == 1 ? (rows + 15) & ~15 : ((rows + tt_e - 1) / tt_e + 31) & ~31;
-    t.t0 = row_start[t.e] + jt * width;
+    t.t0 = row_start[t.e] + (j % tt_e) * F8_ROWS;
     t.n0 = (j / tt_e) * TILE_N;
-    t.n_main = min(width, (t.t_end - t.t0 + 15) & ~15);
+    t.n = GATE_UP ? 256 : min(256, (p.N - t.n0 + 31) & ~31);
+    t.t_end = row_start[t.e + 1];
     return t;
-  };
-  auto small_boxes = [&](int n_main) {  // of this CTA's half of the tokens; 0: one box of 128 rows
-    const int rows = n_main >> 1;
-    return rows <= 64 ? (rows + PAIR_SMALL_BOX - 1) / PAIR_SMALL_BOX : 0;
   };
 
   if (warp < 4) {
@@ -157,6 +163,10 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
       if (elect_one()) {
         Feed feed(&ctl->sched, abort_flag);
         const uint32_t full_leader0 = map_to_cta(smem_u32(&ctl->full[0]), 0);
+        // boxes of a CTA's token rows: one of 128, or as many of 16 as hold rows; rows that are not loaded have sums that
+        // nobody reads
+        auto small_boxes = [&](int rows) { return rows > 64 ? 0 : rows <= 0 ? -1 : (rows + PAIR_SMALL_BOX - 1) / PAIR_SMALL_BOX; };
+        auto box_bytes = [&](int boxes) { return boxes < 0 ? 0 : boxes == 0 ? F8_HALF_BYTES : boxes * PAIR_SMALL_BOX * F8_BK; };
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
@@ -164,26 +174,29 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
           const int tile = feed.take();
           if (tile < 0) break;
           const Fp8Tile t = decode(tile);
-          const int w_row = t.n0 + (int)rank * 128;
-          const int tok = t.t0 + (int)rank * (t.n_main >> 1);
-          const int nsb = small_boxes(t.n_main);
-          const uint32_t b_bytes = nsb ? nsb * PAIR_SMALL_BOX * F8_BK : F8_HALF_BYTES;
+          const int tok = t.t0 + (int)rank * 128;
+          const int nsb = small_boxes(t.t_end - tok);
+          const uint32_t bytes = 2 * F8_HALF_BYTES + box_bytes(small_boxes(t.t_end - t.t0)) + box_bytes(small_boxes(t.t_end - t.t0 - 128));
           for (int i = 0; i < p.n_seg && ok; ++i) {
             for (int kb = 0; kb < p.kb; ++kb) {
               if (!mbar_wait(&ctl->empty[s], ph ^ 1, abort_flag, PW_EMPTY)) { ok = false; break; }
               uint8_t* sa = smem + s * F8_STAGE_BYTES;
               uint8_t* sb = sa + F8_HALF_BYTES;
               const uint32_t bar = full_leader0 + s * 8;
-              if (leader) mbar_expect_tx(&ctl->full[s], 2 * (F8_HALF_BYTES + b_bytes));  // both CTAs' bytes
-              if constexpr (W_MN) tma_load_3d_pair(sa, &maps.w[i], bar, w_row, kb * F8_BK, t.e);
-              else tma_load_3d_pair(sa, &maps.w[i], bar, kb * F8_BK, w_row, t.e);
-              if (nsb == 0) {
-                tma_load_2d_pair(sb, &maps.x[i], bar, kb * F8_BK, tok);
+              if (leader) mbar_expect_tx(&ctl->full[s], bytes);  // both CTAs' bytes
+              if constexpr (GATE_UP) {
+                const int feat = t.n0 + (int)rank * 64;
+                tma_load_3d_pair(sb, &maps.w[0], bar, kb * F8_BK, feat, t.e);
+                tma_load_3d_pair(sb + F8_HALF_BYTES / 2, &maps.w[1], bar, kb * F8_BK, feat, t.e);
               } else {
-                for (int b = 0; b < nsb; ++b)
-                  tma_load_2d_pair(sb + b * (PAIR_SMALL_BOX * F8_BK), &maps.xs[i], bar, kb * F8_BK, tok + b * PAIR_SMALL_BOX);
+                const int w_row = t.n0 + (int)rank * (t.n >> 1);
+                if constexpr (W_MN) tma_load_3d_pair(sb, &maps.w[i], bar, w_row, kb * F8_BK, t.e);
+                else tma_load_3d_pair(sb, &maps.w[i], bar, kb * F8_BK, w_row, t.e);
               }
-              if (++s == F8_STAGES) { s = 0; ph ^= 1; }
+              if (nsb == 0) tma_load_2d_pair(sa, &maps.x[i], bar, kb * F8_BK, tok);
+              for (int b = 0; b < nsb; ++b)
+                tma_load_2d_pair(sa + b * (PAIR_SMALL_BOX * F8_BK), &maps.xs[i], bar, kb * F8_BK, tok + b * PAIR_SMALL_BOX);
+              if (++s == p.stages) { s = 0; ph ^= 1; }
             }
           }
         }
@@ -201,191 +214,262 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         int s = 0;
         uint32_t ph = 0;
         bool ok = true;
-        while (ok) {
-          const int tile = feed.take();
-          if (tile < 0) break;
-          const Fp8Tile t = decode(tile);
-          const uint32_t idesc = p.idesc | ((uint32_t)(t.n_main >> 3) << 17);
+        int tile = feed.take();
+        while (ok && tile >= 0) {
+          const uint32_t idesc = p.idesc | ((uint32_t)(decode(tile).n >> 3) << 17);
           for (int b = 0; b < steps; ++b, ++it) {
             const uint32_t buf = it & 1;
-            if (!mbar_wait_cluster(&ctl->tmem_free[buf], ((it >> 1) & 1) ^ 1, abort_flag, PW_TMEM_EMPTY)) { ok = false; break; }
-            if (!mbar_wait_cluster(&ctl->full[s], ph, abort_flag, PW_FULL)) { ok = false; break; }
+            if (!mbar_wait(&ctl->full[s], ph, abort_flag, PW_FULL)) { ok = false; break; }
+            if (!mbar_wait(&ctl->tmem_free[buf], ((it >> 1) & 1) ^ 1, abort_flag, PW_TMEM_EMPTY)) { ok = false; break; }
             tc_fence_after_sync();
             const uint32_t sa = smem_u32(smem + s * F8_STAGE_BYTES);
-            const uint64_t da = make_smem_desc(sa, W_MN ? F8_HALF_BYTES : 16, 1024);
-            const uint64_t db = make_smem_desc(sa + F8_HALF_BYTES, 16, 1024);
-            const uint32_t d = tmem_base + buf * PAIR_TOKENS;
+            const uint64_t da = make_smem_desc(sa, 16, 1024);
+            const uint64_t db = make_smem_desc(sa + F8_HALF_BYTES, W_MN ? F8_HALF_BYTES : 16, 1024);
+            const uint32_t d = tmem_base + buf * 256;
 #pragma unroll
             for (int k = 0; k < F8_BK / F8_UMMA_K; ++k) {
-              const uint64_t b_adv = (uint64_t)((k * F8_UMMA_K) >> 4);
-              const uint64_t a_adv = W_MN ? (uint64_t)((k * F8_UMMA_K * 128) >> 4) : b_adv;
+              const uint64_t a_adv = (uint64_t)((k * F8_UMMA_K) >> 4);
+              const uint64_t b_adv = W_MN ? (uint64_t)((k * F8_UMMA_K * 128) >> 4) : a_adv;
               umma_f8_pair(d, da + a_adv, db + b_adv, idesc, k != 0);
             }
             umma_commit_pair(&ctl->empty[s], 3);
             umma_commit_pair(&ctl->tmem_full[buf], 3);
-            if (++s == F8_STAGES) { s = 0; ph ^= 1; }
+            if (++s == p.stages) { s = 0; ph ^= 1; }
+            if (b == 0) tile = feed.take();  // the next one, while this tile's blocks are on their way
           }
         }
       }
     } else if (warp == 2) {
-      // ------------------------------ factors (both CTAs) ------------------------------
-      // Four blocks' scales are loaded at a time: a block's MMAs take less time than one trip to memory.
+      // ---------------- tiles for the epilogue (both CTAs): taken from the pair's ring and decoded ----------------
+      // (under the MMAs' operand traffic an access to shared memory takes 100 to 300 cycles, and this chain has a dozen: 3400
+      // cycles of a tile when the epilogue warps did it themselves)
       Feed feed(&ctl->sched, abort_flag);
-      constexpr int AHEAD = 4;
-      uint32_t it = 0;
-      bool ok = true;
-      const int n_blocks = (p.N + 127) / 128;
-      while (ok) {
-        const int tile = feed.take_warp(lane);
-        if (tile < 0) break;
-        const Fp8Tile t = decode(tile);
-        const int nb = min(t.n0 / 128 + (int)rank, n_blocks - 1);
-        const int64_t ws0 = t.e * p.ws_e + (int64_t)nb * p.ws_n;
-        for (int b0 = 0; b0 < steps && ok; b0 += AHEAD) {
-          float v[AHEAD][8], w[AHEAD];
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a) {
-            const int b = b0 + a;
-            const int seg = b >= p.kb ? 1 : 0;
-            const int kb = b - seg * p.kb;
-            if (b < steps) {
-              w[a] = __ldg(p.ws[seg] + ws0 + (int64_t)kb * p.ws_k);
-              const float* src = p.s[seg] + (int64_t)kb * p.M + t.t0;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int col = i * 32 + lane;
-                v[a][i] = col < t.n_main && t.t0 + col < p.M ? __ldg(src + col) : 0.f;
-              }
-            }
+      if (elect_one()) {
+        uint32_t n = 0;
+        while (true) {
+          const int tile = feed.take();
+          int4 info = make_int4(-1, 0, 0, 0);
+          if (tile >= 0) {
+            const Fp8Tile t = decode(tile);
+            info = make_int4(t.e, t.t0, t.n0, t.t_end);
           }
-#pragma unroll
-          for (int a = 0; a < AHEAD; ++a) {
-            if (b0 + a >= steps || !ok) break;
-            const uint32_t q = it % F8_SLOTS, ph = (it / F8_SLOTS) & 1;
-            if (!mbar_wait(&ctl->sempty[q], ph ^ 1, abort_flag, FW_SEMPTY)) { ok = false; break; }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i * 32 < t.n_main) factors[q * 256 + i * 32 + scale_pos(lane)] = v[a][i] * w[a];
-            mbar_arrive(&ctl->sfull[q]);
-            ++it;
-          }
+          const uint32_t q = n % F8_TILES;
+          if (!mbar_wait(&ctl->tile_empty[q], ((n / F8_TILES) & 1) ^ 1, abort_flag, FW_TILE_EMPTY)) break;
+          ctl->tiles[q] = info;
+          mbar_arrive(&ctl->tile_full[q]);
+          if (tile < 0) break;
+          ++n;
         }
       }
     }
   } else {
     // ------------------------------ epilogue (both CTAs) ------------------------------
     registers_inc<F8_EPI_REGS>();
-    Feed feed(&ctl->sched, abort_flag);
     const int quarter = warp & 3;
-    const int wg = (warp >> 2) - 1;
-    const int epi_tid = threadIdx.x & 127;
+    const int wg = (warp >> 2) - 1;       // columns wg * 128 ..
+    const int row = quarter * 32 + lane;  // of this CTA
     const uint32_t tmem_free_leader0 = map_to_cta(smem_u32(&ctl->tmem_free[0]), 0);
-    uint8_t* const my_staging = staging + wg * (4 * PAIR_STAGING_BYTES);
-    const int half = quarter >> 1;
-    const int chunk = 4 * (quarter & 1) + (lane >> 3);  // 16-byte chunk of the 128-byte staging row
-    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const float* my_factors = factors + (lane & 3) * 8;
-    uint32_t it = 0, round = 0;
-    bool ok = true;
+    uint8_t* const my_staging = staging + (warp - 4) * (2 * F8_WARP_STAGING);
+    const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + wg * 128;
+    uint32_t it = 0, n_tile = 0;
+    bool ok = true;  // a warp whose wait was abandoned goes on without waiting to the end of the tile
+    auto take = [&]() {
+      const uint32_t slot = n_tile % F8_TILES;
+      ok = ok && mbar_wait(&ctl->tile_full[slot], (n_tile / F8_TILES) & 1, abort_flag, FW_TILE_FULL);
+      const int4 info = ok ? ctl->tiles[slot] : make_int4(-1, 0, 0, 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->tile_empty[slot]);
+      ++n_tile;
+      return info;
+    };
+    // Factors: s of the thread's token times ws of its columns' block (GATE_UP: of gate and of up).  They are loaded two blocks
+    // ahead, a tile's first ones before the tile in front of it is stored: a trip to L2 takes longer than a block.
+    struct Raw { float s, w0, w1; };
+    const float* sp = p.s[0];
+    const float* wp = p.ws[0];
+    int fetched = 0;
+    auto start = [&](const int4& t) {
+      if (t.x < 0) return;
+      const int nb = GATE_UP ? t.z / 128 : min(t.z / 128 + wg, (p.N - 1) / 128);
+      sp = p.s[0] + min(t.y + (int)rank * 128 + row, t.w - 1);
+      wp = p.ws[0] + t.x * p.ws_e + (int64_t)nb * p.ws_n;
+      fetched = 0;
+    };
+    auto fetch = [&]() {
+      Raw r = {0.f, 0.f, 0.f};
+      if (fetched < steps) {
+        r.s = __ldg(sp);
+        r.w0 = __ldg(wp);
+        if (GATE_UP) r.w1 = __ldg(wp + (p.ws[1] - p.ws[0]));
+        sp += p.pitch;
+        wp += p.ws_k;
+        if (++fetched == p.kb && !GATE_UP) {  // on to the second operand pair
+          sp += (p.s[1] - p.s[0]) - p.kb * p.pitch;
+          wp += (p.ws[1] - p.ws[0]) - (int64_t)p.kb * p.ws_k;
+        }
+      }
+      return r;
+    };
+    int4 info = take();
+    start(info);
+    Raw r0 = fetch(), r1 = fetch();
     while (true) {
-      const int tile = feed.take_warp(lane);
-      // the four warps of a warpgroup leave together; a warp whose wait was abandoned goes on without waiting until here
-      if (named_barrier_any(3 + wg, 128, tile < 0 || !ok)) break;
-      const Fp8Tile t = decode(tile);
-      const int runs = (t.n_main + 31) >> 5;  // of 32 columns; this warp's are wg, wg + 2, ...
+      const bool leave = __any_sync(0xffffffffu, info.x < 0);
+      if constexpr (GATE_UP) {  // the two warps that share tokens leave together
+        if (named_barrier_any(1 + quarter, 64, leave)) break;
+      } else {
+        if (leave) break;
+      }
+      const int t_n0 = info.z;
+      const int tok0 = info.y + (int)rank * 128 + quarter * 32;  // first token of the warp
+      const int rows = info.w - tok0;                            // of the warp's 32 that belong to the expert
+      const bool live = rows > 0;
       uint64_t acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = 0;
-#pragma unroll 1
-      for (int b = 0; b < steps; ++b, ++it) {
-        const uint32_t buf = it & 1, q = it % F8_SLOTS;
-        if (ok) ok = mbar_wait_cluster(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
-        if (ok) ok = mbar_wait(&ctl->sfull[q], (it / F8_SLOTS) & 1, abort_flag, FW_SFULL);
+      auto add_block = [&](const Raw& r) {
+        const uint32_t buf = it & 1;
+        ok = ok && mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
         tc_fence_after_sync();
+        ++it;
+        if (live) {
+          const uint32_t taddr = taddr0 + buf * 256;
+          uint32_t v[32];
+          const uint32_t f0 = __float_as_uint(r.s * r.w0), f1 = GATE_UP ? __float_as_uint(r.s * r.w1) : f0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (2 * i + wg < runs) {
-            const int c = (2 * i + wg) * 32;
-            uint32_t lo[16], hi[16];
-            tmem_ld_16x256b_x4(lane_base + buf * PAIR_TOKENS + c, lo);
-            tmem_ld_16x256b_x4(lane_base + buf * PAIR_TOKENS + c + (16u << 16), hi);
-            const ulonglong2 f0 = *reinterpret_cast<const ulonglong2*>(my_factors + q * 256 + c);
-            const ulonglong2 f1 = *reinterpret_cast<const ulonglong2*>(my_factors + q * 256 + c + 4);
-            const uint64_t f[4] = {f0.x, f0.y, f1.x, f1.y};
-            tmem_ld_wait();
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint64_t* a = acc + i * 16 + g * 4;
-              a[0] = fma_f32x2(pack_f32x2(lo[4 * g], lo[4 * g + 1]), f[g], a[0]);
-              a[1] = fma_f32x2(pack_f32x2(lo[4 * g + 2], lo[4 * g + 3]), f[g], a[1]);
-              a[2] = fma_f32x2(pack_f32x2(hi[4 * g], hi[4 * g + 1]), f[g], a[2]);
-              a[3] = fma_f32x2(pack_f32x2(hi[4 * g + 2], hi[4 * g + 3]), f[g], a[3]);
+          for (int i = 0; i < 4; ++i) {
+            tmem_ld_32x32(taddr + i * 32, v);
+            tmem_ld_wait(v);
+            if (i == 3) {
+              tc_fence_before_sync();
+              if (lane == 0) mbar_arrive_relaxed_cluster(tmem_free_leader0 + buf * 8);  // (the wait above was the whole warp's)
             }
+            const uint64_t ff = i < 2 ? pack_f32x2(f0, f0) : pack_f32x2(f1, f1);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[i * 16 + j] = fma_f32x2(pack_f32x2(v[2 * j], v[2 * j + 1]), ff, acc[i * 16 + j]);
           }
+        } else {
+          if (lane == 0) mbar_arrive_relaxed_cluster(tmem_free_leader0 + buf * 8);
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive_cluster(tmem_free_leader0 + buf * 8);
-          mbar_arrive(&ctl->sempty[q]);
+      };
+#pragma unroll 1
+      for (int b = 0; b < steps; b += 2) {
+        const Raw c0 = r0, c1 = r1;
+        r0 = fetch();
+        add_block(c0);
+        if (b + 1 < steps) {
+          r1 = fetch();
+          add_block(c1);
         }
       }
-      const int n_cta = t.n0 + (int)rank * 128;
-      if (p.dtype_out == MOE_F32) {
-        float* out = reinterpret_cast<float*>(p.out);
+      info = take();
+      start(info);
+      r0 = fetch();
+      r1 = fetch();
+      if constexpr (!GATE_UP) {
+        if (!live) continue;
+        const int n0 = t_n0 + wg * 128;  // first column
+        if (p.dtype_out == MOE_F32) {
+          float* out = reinterpret_cast<float*>(p.out) + (int64_t)(tok0 + lane) * p.N + n0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (2 * i + wg < runs) {
-            const int tok = t.t0 + (2 * i + wg) * 32 + 2 * (lane & 3);
+          for (int j = 0; j < 32; ++j)  // columns end at a multiple of 16
+            if (lane < rows && n0 + j * 4 < p.N)
+              *reinterpret_cast<ulonglong2*>(out + j * 4) = make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
+        } else {
+          const bool is_bf16 = p.dtype_out == MOE_BF16;
+          if (lane == 0) tma_store_wait_read<0>();  // the stores of the tile before have read the buffers
+          __syncwarp();
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+          for (int h = 0; h < 2; ++h) {
+            const int n = n0 + h * 64;
+            uint8_t* buf = my_staging + h * F8_WARP_STAGING;
+            if (n < p.N) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int n = n_cta + quarter * 32 + r * 8 + (lane >> 2);
-                const uint64_t v = acc[i * 16 + g * 4 + r];
-                if (n < p.N && tok + 8 * g < t.t_end) out[(int64_t)(tok + 8 * g) * p.N + n] = lo_f32(v);
-                if (n < p.N && tok + 8 * g + 1 < t.t_end) out[(int64_t)(tok + 8 * g + 1) * p.N + n] = hi_f32(v);
+              for (int c = 0; c < 8; ++c) {  // 16 bytes: 8 columns
+                uint32_t m[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  const uint64_t a = acc[h * 32 + c * 4 + r];
+                  m[r] = is_bf16 ? pack2<__nv_bfloat16>(lo_f32(a), hi_f32(a)) : pack2<__half>(lo_f32(a), hi_f32(a));
+                }
+                *reinterpret_cast<uint4*>(buf + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(m[0], m[1], m[2], m[3]);
               }
+            }
+          }
+          if (rows >= 32) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (n0 < p.N) tma_store_2d(&maps.out, my_staging, n0, tok0);  // columns past N are clipped
+              if (n0 + 64 < p.N) tma_store_2d(&maps.out, my_staging + F8_WARP_STAGING, n0 + 64, tok0);
+              tma_store_commit();
+            }
+          } else {
+            __syncwarp();
+            uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
+            for (int i = lane; i < rows * 16; i += 32) {
+              const int r = i >> 4, c = i & 15;
+              if (n0 + c * 8 < p.N)
+                *reinterpret_cast<uint4*>(out + ((int64_t)(tok0 + r) * p.N + n0 + c * 8) * 2) =
+                    *reinterpret_cast<const uint4*>(my_staging + (c >> 3) * F8_WARP_STAGING + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            }
+            __syncwarp();
           }
         }
       } else {
-        const bool is_bf16 = p.dtype_out == MOE_BF16;
+        if (!live) continue;  // (the same for the two warps that share the tokens)
+        const int tok = tok0 + lane, f0 = t_n0 + wg * 64;
+        const bool mine = lane < rows;
+        if (p.keep_e != nullptr && mine) {
+          const bool is_bf16 = p.dtype_out == MOE_BF16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (2 * i + wg < runs) {
-            const int c = (2 * i + wg) * 32;
-            uint8_t* buf = my_staging + (round & 1) * (2 * PAIR_STAGING_BYTES);
-            ++round;
-            if (epi_tid == 0) tma_store_wait_read<1>();  // the stores of two rounds ago have read this buffer
-            named_barrier_sync(1 + wg, 128);
-            uint8_t* tile_buf = buf + half * PAIR_STAGING_BYTES;
+          for (int c = 0; c < 8; ++c) {
+            if (f0 + c * 8 < p.N) {  // features end at a multiple of 16
+              uint32_t m[8];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
+              for (int r = 0; r < 8; ++r) {
+                const uint64_t a = acc[(r >> 2) * 32 + c * 4 + (r & 3)];
+                m[r] = is_bf16 ? pack2<__nv_bfloat16>(lo_f32(a), hi_f32(a)) : pack2<__half>(lo_f32(a), hi_f32(a));
+              }
+              const int64_t at = ((int64_t)tok * p.N + f0 + c * 8) * 2;
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.keep_e) + at) = make_uint4(m[0], m[1], m[2], m[3]);
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(p.keep_g) + at) = make_uint4(m[4], m[5], m[6], m[7]);
+            }
+          }
+        }
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {  // (features past the last one have zeros in both)
+          const float h0 = gated_silu(lo_f32(acc[i]), lo_f32(acc[32 + i])), h1 = gated_silu(hi_f32(acc[i]), hi_f32(acc[32 + i]));
+          top = max(top, max(magnitude_bits(h0), magnitude_bits(h1)));
+          acc[i] = pack_f32x2(__float_as_uint(h0), __float_as_uint(h1));
+        }
+        // the scale's other 64 features are with the other warpgroup; the next tile's words are written behind the vote above
+        uint32_t* tops = reinterpret_cast<uint32_t*>(staging);
+        tops[wg * 128 + row] = top;
+        named_barrier_sync(1 + quarter, 64);
+        top = max(top, tops[(wg ^ 1) * 128 + row]);
+        float inv;
+        const float scale = fp8_block_scale(top, inv);
+        if (mine) {
+          if (wg == 0) p.out_s[(int64_t)(t_n0 / 128) * p.pitch + tok] = scale;
+          uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + (int64_t)tok * p.N + f0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (f0 + c * 16 < p.N) {
               uint32_t m[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const uint64_t v = acc[i * 16 + g * 4 + r];
-                m[r] = is_bf16 ? pack2<__nv_bfloat16>(lo_f32(v), hi_f32(v)) : pack2<__half>(lo_f32(v), hi_f32(v));
+                const uint64_t a = acc[c * 8 + r * 2], b = acc[c * 8 + r * 2 + 1];
+                m[r] = fp8_pack4(lo_f32(a) * inv, hi_f32(a) * inv, lo_f32(b) * inv, hi_f32(b) * inv);
               }
-              const int trow = 8 * g + (lane & 7);
-              stmatrix_x4_trans(smem_u32(tile_buf + trow * 128 + ((chunk ^ (trow & 7)) << 4)), m[0], m[1], m[2], m[3]);
-            }
-            fence_proxy_async_smem();
-            named_barrier_sync(1 + wg, 128);
-            const bool clip = t.t_end - (t.t0 + c) < 32;
-            if (clip) store_clipped_rows<16>(buf, reinterpret_cast<uint8_t*>(p.out), t.t0 + c, t.t_end, n_cta, p.N, epi_tid);
-            if (epi_tid == 0) {
-              if (!clip && n_cta < p.N) {
-                tma_store_2d(&maps.out, buf, n_cta, t.t0 + c);
-                if (n_cta + 64 < p.N) tma_store_2d(&maps.out, buf + PAIR_STAGING_BYTES, n_cta + 64, t.t0 + c);
-              }
-              tma_store_commit();
+              *reinterpret_cast<uint4*>(out + c * 16) = make_uint4(m[0], m[1], m[2], m[3]);
             }
           }
         }
       }
     }
-    if (epi_tid == 0) tma_store_wait_all();
+    if (lane == 0) tma_store_wait_all();
   }
 
   tc_fence_before_sync();

@@ -50,6 +50,7 @@ SIGNATURES = {
     "moe_absmax_unnest": (_I, [_P, _P, _P, _I, _P, _P, _L, _P]),
     "moe_fp8_quantize_rows": (_I, [_P, _I, _L, _I, _P, _P, _P]),
     "moe_grouped_gemm_fp8": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _P]),
+    "moe_gate_up_silu_fp8": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P]),
     "moe_fp8_silu_quantize": (_I, [_P, _P, _L, _I, _P, _P, _P, _P, _I, _P]),
     "moe_fp8_silu_bwd_quantize": (_I, [_P, _P, _P, _L, _I, _P, _P, _P, _P, _I, _P]),
     "moe_silu_mul_fwd": (_I, [_P, _P, _P, _L, _I, _P]),

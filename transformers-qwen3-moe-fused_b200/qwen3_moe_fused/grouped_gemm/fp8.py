@@ -19,7 +19,8 @@ def grouped_gemm_fp8(pairs, m_sizes: torch.Tensor, dtype: torch.dtype, transpose
         check_weight(w, ws)
         assert w.shape == ((E, K, N) if transposed else (E, N, K)) and w.device == q0.device
         assert q.shape == (M, K) and q.dtype == FP8 and q.is_contiguous() and q.device == q0.device
-        assert s.shape == (blocks(K), M) and s.dtype == torch.float32 and s.is_contiguous() and s.device == q0.device
+        assert s.shape == (blocks(K), M) and s.dtype == torch.float32 and s.device == q0.device
+        assert (M <= 1 or s.stride(1) == 1) and (s.shape[0] == 1 or M == 0 or s.stride(0) == -(-M // 4) * 4)
         args += [_lib.ptr(q), _lib.ptr(s), _lib.ptr(w), _lib.ptr(ws)]
     args += [None] * (8 - len(args))
     m_sizes = _lib.as_index_tensor(m_sizes)

@@ -13,24 +13,40 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ..grouped_gemm.fp8 import grouped_gemm_fp8
-from ..quantize.fp8 import FP8, blocks, quantize_fp8_rows
+from ..quantize.fp8 import FP8, check_weight, empty_scales, quantize_fp8_rows
 
 
 def _codes(M: int, K: int, device):
-    return torch.empty((M, K), device=device, dtype=FP8), torch.empty((blocks(K), M), device=device, dtype=torch.float32)
+    return torch.empty((M, K), device=device, dtype=FP8), empty_scales(M, K, device)
 
 
 def _gate_up(x, gate, gate_scale, up, up_scale, m_sizes, keep: bool):
     """(hq, hs) and, with `keep`, (e, g) in the type of x."""
     q, s = quantize_fp8_rows(x)
-    M, I = x.shape[0], gate.shape[1]
-    e32 = grouped_gemm_fp8(((q, s, gate, gate_scale),), m_sizes, torch.float32)
-    g32 = grouped_gemm_fp8(((q, s, up, up_scale),), m_sizes, torch.float32)
+    M, K = x.shape
+    E, I = gate.shape[:2]
+    check_weight(gate, gate_scale)
+    check_weight(up, up_scale)
+    assert gate.shape[2] == K and gate.device == up.device == m_sizes.device == x.device
+    assert m_sizes.ndim == 1 and m_sizes.is_contiguous() and m_sizes.numel() == E and _lib.is_int_tensor(m_sizes)
+    ms = _lib.as_index_tensor(m_sizes)
     hq, hs = _codes(M, I, x.device)
     e, g = (torch.empty((M, I), device=x.device, dtype=x.dtype) if keep else None for _ in range(2))
+    lib = _lib.load()
     with torch.cuda.device(x.device):
-        status = _lib.load().moe_fp8_silu_quantize(_lib.ptr(e32), _lib.ptr(g32), M, I, _lib.ptr(hq), _lib.ptr(hs), _lib.ptr(e),
-                                                   _lib.ptr(g), _lib.float_code(x.dtype), _lib.stream_ptr(x.device))
+        status = lib.moe_gate_up_silu_fp8(
+            _lib.ptr(q), _lib.ptr(s), _lib.ptr(gate), _lib.ptr(gate_scale), _lib.ptr(up), _lib.ptr(up_scale), _lib.ptr(ms),
+            _lib.int_code(ms.dtype), _lib.ptr(hq), _lib.ptr(hs), _lib.ptr(e), _lib.ptr(g), M, I, K, E, _lib.float_code(x.dtype),
+            _lib.stream_ptr(x.device))
+    if status != _lib.ERR_UNSUPPORTED:
+        _lib.check(status, "moe_gate_up_silu_fp8")
+        return hq, hs, e, g
+    # extents or types that the kernel does not cover: the products one by one
+    e32 = grouped_gemm_fp8(((q, s, gate, gate_scale),), m_sizes, torch.float32)
+    g32 = grouped_gemm_fp8(((q, s, up, up_scale),), m_sizes, torch.float32)
+    with torch.cuda.device(x.device):
+        status = lib.moe_fp8_silu_quantize(_lib.ptr(e32), _lib.ptr(g32), M, I, _lib.ptr(hq), _lib.ptr(hs), _lib.ptr(e), _lib.ptr(g),
+                                           _lib.float_code(x.dtype), _lib.stream_ptr(x.device))
     _lib.check(status, "moe_fp8_silu_quantize")
     return hq, hs, e, g
 

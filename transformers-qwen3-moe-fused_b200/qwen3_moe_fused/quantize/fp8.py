@@ -55,13 +55,18 @@ def check_weight(codes: torch.Tensor, scale: torch.Tensor) -> None:
     assert scale.shape == (codes.shape[0], blocks(codes.shape[1]), blocks(codes.shape[2]))
 
 
+def empty_scales(M: int, K: int, device) -> torch.Tensor:
+    """(ceil(K / 128), M) with rows padded to a multiple of 4, as the kernels lay them out."""
+    return torch.empty((blocks(K), -(-M // 4) * 4), device=device, dtype=torch.float32)[:, :M]
+
+
 @torch.no_grad()
 def quantize_fp8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes (M, K), scale (ceil(K / 128), M)) of activations x (M, K): x[m, k] is about codes[m, k] * scale[k // 128, m]."""
     assert x.is_cuda and x.ndim == 2 and x.is_contiguous() and x.shape[1] >= 1
     M, K = x.shape
     q = torch.empty((M, K), device=x.device, dtype=FP8)
-    s = torch.empty((blocks(K), M), device=x.device, dtype=torch.float32)
+    s = empty_scales(M, K, x.device)
     with torch.cuda.device(x.device):
         status = _lib.load().moe_fp8_quantize_rows(_lib.ptr(x), _lib.float_code(x.dtype), M, K, _lib.ptr(q), _lib.ptr(s),
                                                    _lib.stream_ptr(x.device))
