@@ -57,7 +57,7 @@ inline int sm_count() {
 }
 
 // Elements between the blocks of the scales of M quantised rows: whole 16-byte units, as the copy engine wants them.
-inline int64_t fp8_scale_pitch(int64_t M) { return (M + 3) & ~(int64_t)3; }
+__host__ __device__ inline int64_t fp8_scale_pitch(int64_t M) { return (M + 3) & ~(int64_t)3; }
 
 // moe_grouped_gemm_sum whose product i counts 2^log2_scale[i] times (null: once; at most 2^15 between any two), and
 // moe_grouped_gemm_dw_strided whose gradients are multiplied by alpha / alpha2 ahead of their rounding (gemm_api.cu).

@@ -25,33 +25,11 @@ namespace {
 
 constexpr int Q_THREADS = 256;
 
-// Half a warp owns 128 values of a row: 8 consecutive ones in each lane, loaded through `load(row, col, v)` (col < K; lanes
-// past the row's end get zeros), the largest magnitude by shuffles, 8 codes stored as one word of 8 bytes.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int col, int K, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (col < K) {
-#pragma unroll
-      for (int i = 0; i < 8; i += Vec<T>::N) {
-        const Vec<T> r = load_vec(row + col + i);
-#pragma unroll
-        for (int j = 0; j < Vec<T>::N; ++j) v[i + j] = to_f32(r.v[j]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < K ? to_f32(row[col + i]) : 0.f;
-  }
-}
-
+// Half a warp owns 128 values of a row, 8 consecutive ones in each lane (zeros past the row's end): the largest magnitude by
+// shuffles, 8 codes stored as one word of 8 bytes.
+// `top`: the bits of the lane's largest magnitude.
 template <bool VEC>
-__device__ __forceinline__ void store_codes(const float (&v)[8], uint8_t* row, int col, int K, float* scale) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(v[i]));
+__device__ __forceinline__ void store_codes(const float (&v)[8], uint32_t top, uint8_t* row, int col, int K, float* scale) {
 #pragma unroll
   for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
   float inv;
@@ -69,28 +47,86 @@ __device__ __forceinline__ void store_codes(const float (&v)[8], uint8_t* row, i
   }
 }
 
-// Items are (row, pair of blocks); a warp takes one item per step.
-template <typename Body>
-__device__ __forceinline__ void for_row_blocks(int64_t M, int K, Body body) {
-  const int pairs = (K + 2 * FP8_BLOCK - 1) / (2 * FP8_BLOCK);
+// A warp takes UNROLL neighbouring pairs of blocks of a row (blockIdx.y: which of them) and loads all before it works on the
+// first one.
+struct RowBlock {
+  int64_t row;
+  int col, kb;
+};
+template <int UNROLL, typename Values, typename Load, typename Work>
+__device__ __forceinline__ void for_row_blocks(int64_t M, int K, Load load, Work work) {
   const int lane = threadIdx.x & 31;
-  const int64_t warps = (int64_t)gridDim.x * (Q_THREADS / 32);
-  for (int64_t i = (int64_t)blockIdx.x * (Q_THREADS / 32) + (threadIdx.x >> 5); i < M * pairs; i += warps) {
-    const int64_t row = i / pairs;
-    const int p = (int)(i % pairs);
-    body(row, p * 2 * FP8_BLOCK + lane * 8, 2 * p + (lane >> 4));
+  const int p0 = blockIdx.y * UNROLL;
+  const int64_t step = (int64_t)gridDim.x * (Q_THREADS / 32);
+  for (int64_t row = (int64_t)blockIdx.x * (Q_THREADS / 32) + (threadIdx.x >> 5); row < M; row += step) {
+    Values v[UNROLL];
+    auto at = [&](int u) { return RowBlock{row, (p0 + u) * 2 * FP8_BLOCK + lane * 8, 2 * (p0 + u) + (lane >> 4)}; };
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) load(at(u), v[u]);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if ((p0 + u) * 2 * FP8_BLOCK < K) work(at(u), v[u]);  // (the same for the whole warp)
   }
 }
 
+// Eight consecutive values as they are in memory.
 template <typename T, bool VEC>
+struct alignas(16) Eight {
+  T v[8];
+  __device__ __forceinline__ void load(const T* row, int col, int K) {
+    if constexpr (VEC) {
+      constexpr int WORDS = 8 * sizeof(T) / 16;
+      uint4* to = reinterpret_cast<uint4*>(v);
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) to[i] = col < K ? __ldcs(reinterpret_cast<const uint4*>(row + col) + i) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = col + i < K ? row[col + i] : from_f32<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(v[i]);
+  }
+  // Bits of the largest magnitude as fp32.  16-bit types: two at a time, as integers (infinity and NaN above all numbers).
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (VEC && sizeof(T) == 2) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+      uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      const uint16_t big = (uint16_t)max(m & 0xffffu, m >> 16);
+      T t;
+      *reinterpret_cast<uint16_t*>(&t) = big;
+      return magnitude_bits(to_f32(t));
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, magnitude_bits(to_f32(v[i])));
+      return m;
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t top_of(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, magnitude_bits(f[i]));
+  return m;
+}
+
+template <typename T, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(Q_THREADS)
 quantize_rows_kernel(const T* __restrict__ x, int64_t M, int K, uint8_t* __restrict__ q, float* __restrict__ scale) {
-  const int64_t pitch = (M + 3) & ~(int64_t)3;
-  for_row_blocks(M, K, [&](int64_t row, int col, int kb) {
-    float v[8];
-    load8<T, VEC>(x + row * K, col, K, v);
-    store_codes<VEC>(v, q + row * K, col, K, scale + kb * pitch + row);
-  });
+  const int64_t pitch = fp8_scale_pitch(M);
+  using Values = Eight<T, VEC>;
+  for_row_blocks<UNROLL, Values>(M, K,
+    [&](const RowBlock& at, Values& v) { v.load(x + at.row * K, at.col, K); },
+    [&](const RowBlock& at, const Values& v) {
+      float f[8];
+      v.get(f);
+      store_codes<VEC>(f, v.top(), q + at.row * K, at.col, K, scale + at.kb * pitch + at.row);
+    });
 }
 
 // h = silu(e) g of two fp32 products, quantised; e and g are kept in T for a backward pass (keep_e, keep_g, may be null).
@@ -98,21 +134,25 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 silu_quantize_kernel(const float* __restrict__ e, const float* __restrict__ g, int64_t M, int I, uint8_t* __restrict__ hq,
                      float* __restrict__ hs, T* __restrict__ keep_e, T* __restrict__ keep_g) {
-  const int64_t pitch = (M + 3) & ~(int64_t)3;
-  for_row_blocks(M, I, [&](int64_t row, int col, int kb) {
-    float ve[8], vg[8], h[8];
-    load8<float, VEC>(e + row * I, col, I, ve);
-    load8<float, VEC>(g + row * I, col, I, vg);
+  const int64_t pitch = fp8_scale_pitch(M);
+  struct Values { Eight<float, VEC> e, g; };
+  for_row_blocks<1, Values>(M, I,
+    [&](const RowBlock& at, Values& v) {
+      v.e.load(e + at.row * I, at.col, I);
+      v.g.load(g + at.row * I, at.col, I);
+    },
+    [&](const RowBlock& at, const Values& v) {
+      float h[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[i] = gated_silu(ve[i], vg[i]);
-      if (keep_e && col + i < I) {
-        keep_e[row * I + col + i] = from_f32<T>(ve[i]);
-        keep_g[row * I + col + i] = from_f32<T>(vg[i]);
+      for (int i = 0; i < 8; ++i) {
+        h[i] = gated_silu(v.e.v[i], v.g.v[i]);
+        if (keep_e && at.col + i < I) {
+          keep_e[at.row * I + at.col + i] = from_f32<T>(v.e.v[i]);
+          keep_g[at.row * I + at.col + i] = from_f32<T>(v.g.v[i]);
+        }
       }
-    }
-    store_codes<VEC>(h, hq + row * I, col, I, hs + kb * pitch + row);
-  });
+      store_codes<VEC>(h, top_of(h), hq + at.row * I, at.col, I, hs + at.kb * pitch + at.row);
+    });
 }
 
 // Gradients of e and g from the fp32 gradient of h, quantised.
@@ -120,17 +160,21 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 silu_bwd_quantize_kernel(const float* __restrict__ dh, const T* __restrict__ e, const T* __restrict__ g, int64_t M, int I,
                          uint8_t* __restrict__ deq, float* __restrict__ des, uint8_t* __restrict__ dgq, float* __restrict__ dgs) {
-  const int64_t pitch = (M + 3) & ~(int64_t)3;
-  for_row_blocks(M, I, [&](int64_t row, int col, int kb) {
-    float vd[8], ve[8], vg[8];
-    load8<float, VEC>(dh + row * I, col, I, vd);
-    load8<T, VEC>(e + row * I, col, I, ve);
-    load8<T, VEC>(g + row * I, col, I, vg);
+  const int64_t pitch = fp8_scale_pitch(M);
+  struct Values { Eight<float, VEC> dh; Eight<T, VEC> e, g; };
+  for_row_blocks<VEC ? 2 : 1, Values>(M, I,
+    [&](const RowBlock& at, Values& v) {
+      v.dh.load(dh + at.row * I, at.col, I);
+      v.e.load(e + at.row * I, at.col, I);
+      v.g.load(g + at.row * I, at.col, I);
+    },
+    [&](const RowBlock& at, const Values& v) {
+      float de[8], dg[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) gated_silu_bwd(vd[i], ve[i], vg[i], ve[i], vg[i]);
-    store_codes<VEC>(ve, deq + row * I, col, I, des + kb * pitch + row);
-    store_codes<VEC>(vg, dgq + row * I, col, I, dgs + kb * pitch + row);
-  });
+      for (int i = 0; i < 8; ++i) gated_silu_bwd(v.dh.v[i], to_f32(v.e.v[i]), to_f32(v.g.v[i]), de[i], dg[i]);
+      store_codes<VEC>(de, top_of(de), deq + at.row * I, at.col, I, des + at.kb * pitch + at.row);
+      store_codes<VEC>(dg, top_of(dg), dgq + at.row * I, at.col, I, dgs + at.kb * pitch + at.row);
+    });
 }
 
 // ---------------------------------------------------------------------------------------
@@ -210,7 +254,7 @@ simt_gemm_fp8_kernel(const Fp8Pairs ops, const void* m_sizes, int ms64, T* __res
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int64_t t = t0 + ty * 4 + u;
-          const float sx = t < row_end ? ops.s[i][kb * ((M + 3) & ~(int64_t)3) + t] * sw : 0.f;
+          const float sx = t < row_end ? ops.s[i][kb * fp8_scale_pitch(M) + t] * sw : 0.f;
 #pragma unroll
           for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(part[u][v], sx, acc[u][v]);
         }
@@ -228,15 +272,15 @@ simt_gemm_fp8_kernel(const Fp8Pairs ops, const void* m_sizes, int ms64, T* __res
   }
 }
 
-int quantize_grid(int64_t M, int K) {
-  const int64_t items = M * ((K + 2 * FP8_BLOCK - 1) / (2 * FP8_BLOCK));
-  const int64_t want = (items + Q_THREADS / 32 - 1) / (Q_THREADS / 32), cap = (int64_t)sm_count() * 8;
-  return (int)(want < cap ? want : cap);
+dim3 quantize_grid(int64_t M, int K, int unroll) {
+  const int64_t pairs = (K + 2 * FP8_BLOCK - 1) / (2 * FP8_BLOCK), groups = (pairs + unroll - 1) / unroll;
+  const int64_t want = (M + Q_THREADS / 32 - 1) / (Q_THREADS / 32), cap = (int64_t)sm_count() * 16 / groups + 1;
+  return dim3((unsigned)(want < cap ? want : cap), (unsigned)groups);
 }
 
 bool aligned8(const void* p) { return ((uintptr_t)p & 7) == 0; }
 
-bool rows_ok(int64_t M, int K) { return M >= 0 && M <= 0x7fffffffLL && K >= 1; }
+bool rows_ok(int64_t M, int K) { return M >= 0 && M <= 0x7fffffffLL && K >= 1 && K <= 1 << 24; }  // (K: the grid's second extent)
 
 }  // namespace
 }  // namespace moe
@@ -251,8 +295,13 @@ MOE_API int moe_fp8_quantize_rows(const void* x, int dtype, int64_t M, int K, vo
   if (!x || !q || !scale) return MOE_ERR_NULL;
   const bool vec = K % 8 == 0 && aligned16(x) && aligned8(q);
   MOE_DISPATCH_FLOAT(dtype, T, {
-    if (vec) quantize_rows_kernel<T, true><<<quantize_grid(M, K), Q_THREADS, 0, stream>>>((const T*)x, M, K, (uint8_t*)q, scale);
-    else quantize_rows_kernel<T, false><<<quantize_grid(M, K), Q_THREADS, 0, stream>>>((const T*)x, M, K, (uint8_t*)q, scale);
+    // four pairs of blocks to a warp, or three where that leaves fewer of them idle (K = 768: 39 us with four, 65536 rows)
+    const int pairs = (K + 2 * FP8_BLOCK - 1) / (2 * FP8_BLOCK);
+    const int u = !vec ? 1 : (pairs + 2) / 3 * 3 < (pairs + 3) / 4 * 4 ? 3 : 4;
+    const dim3 grid = quantize_grid(M, K, u);
+    if (u == 4) quantize_rows_kernel<T, true, 4><<<grid, Q_THREADS, 0, stream>>>((const T*)x, M, K, (uint8_t*)q, scale);
+    else if (u == 3) quantize_rows_kernel<T, true, 3><<<grid, Q_THREADS, 0, stream>>>((const T*)x, M, K, (uint8_t*)q, scale);
+    else quantize_rows_kernel<T, false, 1><<<grid, Q_THREADS, 0, stream>>>((const T*)x, M, K, (uint8_t*)q, scale);
   });
   return launch_status();
 }
@@ -265,7 +314,7 @@ MOE_API int moe_fp8_silu_quantize(const float* e, const float* g, int64_t M, int
   if (M == 0) return MOE_OK;
   if (!e || !g || !hq || !hs || !keep_e != !keep_g) return MOE_ERR_NULL;
   const bool vec = I % 8 == 0 && aligned16(e) && aligned16(g) && aligned8(hq);
-  const int grid = quantize_grid(M, I);
+  const dim3 grid = quantize_grid(M, I, 1);
   MOE_DISPATCH_FLOAT(dtype, T, {
     if (vec) silu_quantize_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>(e, g, M, I, (uint8_t*)hq, hs, (T*)keep_e, (T*)keep_g);
     else silu_quantize_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>(e, g, M, I, (uint8_t*)hq, hs, (T*)keep_e, (T*)keep_g);
@@ -281,7 +330,7 @@ MOE_API int moe_fp8_silu_bwd_quantize(const float* dh, const void* e, const void
   if (M == 0) return MOE_OK;
   if (!dh || !e || !g || !deq || !des || !dgq || !dgs) return MOE_ERR_NULL;
   const bool vec = I % 8 == 0 && aligned16(dh) && aligned16(e) && aligned16(g) && aligned8(deq) && aligned8(dgq);
-  const int grid = quantize_grid(M, I);
+  const dim3 grid = quantize_grid(M, I, vec ? 2 : 1);
   MOE_DISPATCH_FLOAT(dtype, T, {
     if (vec) silu_bwd_quantize_kernel<T, true><<<grid, Q_THREADS, 0, stream>>>(dh, (const T*)e, (const T*)g, M, I, (uint8_t*)deq, des, (uint8_t*)dgq, dgs);
     else silu_bwd_quantize_kernel<T, false><<<grid, Q_THREADS, 0, stream>>>(dh, (const T*)e, (const T*)g, M, I, (uint8_t*)deq, des, (uint8_t*)dgq, dgs);

@@ -21,7 +21,7 @@ namespace {
 constexpr int NORM_THREADS = 256;    // most threads of a CTA
 constexpr int NORM_MAX_VPT = 4;      // vectors of 16 bytes that a thread keeps of a row
 constexpr int NORM_MAX_H = 24576;    // the generic form keeps two fp32 rows in shared memory
-constexpr int NORM_BWD_CTAS_PER_SM = 4;
+constexpr int NORM_BWD_CTAS_PER_SM = 5;  // at most; the rows of partial sums are laid out for that many
 
 struct NormFwd {
   const void* y;
@@ -200,9 +200,17 @@ norm_fwd_generic_kernel(const NormFwd p) {
 // ---------------------------------------------------------------------------------------
 // backward
 // ---------------------------------------------------------------------------------------
-template <typename T, int VPT>
-__global__ void __launch_bounds__(NORM_THREADS)
+enum NormBwdForm { BWD_ADD = 0, BWD_COMBINE = 1, BWD_COMBINE8 = 2 };  // no expert rows; any k; k = 8 with one vector in each thread
+
+// CTAs that fit on an SM with the registers their form needs.  BWD_COMBINE8 loads the expert rows together with the gradients,
+// ahead of the first sum over the CTA (k = 8, H = 2048, 8191 tokens: 180 us with the rows behind that sum and two CTAs to an SM).
+template <int VPT, int FORM>
+constexpr int norm_bwd_ctas() { return FORM == BWD_ADD ? (VPT == 1 ? 5 : VPT == 2 ? 3 : 1) : FORM == BWD_COMBINE8 ? 3 : (VPT == 1 ? 2 : 1); }
+
+template <typename T, int VPT, int FORM>
+__global__ void __launch_bounds__(NORM_THREADS, norm_bwd_ctas<VPT, FORM>())
 norm_bwd_kernel(const NormBwd p) {
+  static_assert(FORM != BWD_COMBINE8 || VPT == 1, "the loaded rows stay in registers");
   constexpr int V = Vec<T>::N;
   __shared__ float red[2][NORM_THREADS / 32];
   __shared__ float dots[2][NORM_THREADS / 32][8];
@@ -215,17 +223,43 @@ norm_bwd_kernel(const NormBwd p) {
 #pragma unroll
     for (int q = 0; q < V; ++q) dg[i][q] = 0.f;
   int flip = 0, dflip = 0;
+  // dweights of rows j0.. of token t from this thread's products with them
+  auto store_dots = [&](float (&dot)[8], int64_t t, int j0, int nj) {
+    const float v = warp_sum8(dot, lane);
+    if (lane < 8) dots[dflip][warp][lane] = v;
+    __syncthreads();
+    if ((int)threadIdx.x < nj) {
+      float sum = 0.f;
+      for (int w = 0; w < warps; ++w) sum += dots[dflip][w][threadIdx.x];
+      ((T*)p.dweights)[t * p.k + j0 + threadIdx.x] = from_f32<T>(p.scale * sum);
+    }
+    dflip ^= 1;  // written again two rounds on, behind the __syncthreads of the round between
+  };
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     float ds[VPT][V];  // first a, then the gradient of the sum
-    Vec<T> sv[VPT];
+    Vec<T> sv[VPT], d0[VPT];
+    Vec<T> rows[FORM == BWD_COMBINE8 ? 8 : 1];
+    int32_t idx[FORM == BWD_COMBINE8 ? 8 : 1];
+    if constexpr (FORM == BWD_COMBINE8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) idx[j] = p.inv[t * 8 + j];
+      if (p.dweights && (int)threadIdx.x < hv) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(rows[j].v) = __ldcs(reinterpret_cast<const uint4*>(y + (int64_t)idx[j] * p.H) + threadIdx.x);
+      }
+    }
     const float rstd = p.dnormed ? p.rstd[t] : 0.f;
     float au = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
-      if (c >= hv || !p.dnormed) continue;
-      const Vec<T> dn = load_vec((const T*)p.dnormed + t * p.H + c * V);
-      sv[i] = load_vec((const T*)p.sum + t * p.H + c * V);
+      if (c >= hv) continue;
+      if (p.dsum) *reinterpret_cast<uint4*>(d0[i].v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.dsum + t * p.H) + c);
+      if (!p.dnormed) continue;
+      Vec<T> dn;
+      *reinterpret_cast<uint4*>(dn.v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.dnormed + t * p.H) + c);
+      *reinterpret_cast<uint4*>(sv[i].v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.sum + t * p.H) + c);
       const Vec<T> g = load_vec((const T*)p.gamma + c * V);
 #pragma unroll
       for (int q = 0; q < V; ++q) {
@@ -243,60 +277,71 @@ norm_bwd_kernel(const NormBwd p) {
     for (int i = 0; i < VPT; ++i) {
       const int c = threadIdx.x + i * blockDim.x;
       if (c >= hv) continue;
-      Vec<T> d0;
-      if (p.dsum) d0 = load_vec((const T*)p.dsum + t * p.H + c * V);
       Vec<T> o, ox;
 #pragma unroll
       for (int q = 0; q < V; ++q) {
-        float v = p.dsum ? to_f32(d0.v[q]) : 0.f;
+        float v = p.dsum ? to_f32(d0[i].v[q]) : 0.f;
         if (p.dnormed) v = fmaf(rstd, ds[i][q] - to_f32(sv[i].v[q]) * rstd * au, v);
         ds[i][q] = v;
         o.v[q] = from_f32<T>(v);
         ox.v[q] = from_f32<T>(p.scale * v);
       }
-      if (p.dresidual) store_vec((T*)p.dresidual + t * p.H + c * V, o);
-      if (!p.inv && p.dy) store_vec((T*)p.dy + t * p.H + c * V, ox);
+      if (p.dresidual) __stcs(reinterpret_cast<uint4*>((T*)p.dresidual + t * p.H) + c, *reinterpret_cast<const uint4*>(o.v));
+      if (FORM == BWD_ADD && p.dy) __stcs(reinterpret_cast<uint4*>((T*)p.dy + t * p.H) + c, *reinterpret_cast<const uint4*>(ox.v));
     }
-    if (!p.inv || (!p.dy && !p.dweights)) continue;
-    for (int j0 = 0; j0 < p.k; j0 += 8) {
-      const int nj = min(8, p.k - j0);
+    if constexpr (FORM == BWD_COMBINE8) {
+      if (!p.dy && !p.dweights) continue;
       float dot[8];
+      const bool mine = (int)threadIdx.x < hv;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot[j] = 0.f;
+      for (int j = 0; j < 8; ++j) {
+        dot[j] = 0.f;
+        if (!mine) continue;
+        if (p.dweights) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = threadIdx.x + i * blockDim.x;
-        if (c >= hv) continue;
-        Vec<T> v[8];
-        int64_t r[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          r[j] = j < nj ? p.inv[t * p.k + j0 + j] : 0;
-          if (j < nj && p.dweights) *reinterpret_cast<uint4*>(v[j].v) = __ldcs(reinterpret_cast<const uint4*>(y + r[j] * p.H) + c);
+          for (int q = 0; q < V; ++q) dot[j] = fmaf(ds[0][q], to_f32(rows[j].v[q]), dot[j]);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (j >= nj) continue;
-          const float w = p.dy ? p.scale * to_f32(((const T*)p.weights)[t * p.k + j0 + j]) : 0.f;
+        if (p.dy) {
+          const float w = p.scale * to_f32(((const T*)p.weights)[t * 8 + j]);
           Vec<T> o;
 #pragma unroll
-          for (int q = 0; q < V; ++q) {
-            if (p.dweights) dot[j] = fmaf(ds[i][q], to_f32(v[j].v[q]), dot[j]);
-            o.v[q] = from_f32<T>(w * ds[i][q]);
-          }
-          if (p.dy) __stcs(reinterpret_cast<uint4*>((T*)p.dy + r[j] * p.H) + c, *reinterpret_cast<const uint4*>(o.v));
+          for (int q = 0; q < V; ++q) o.v[q] = from_f32<T>(w * ds[0][q]);
+          __stcs(reinterpret_cast<uint4*>((T*)p.dy + (int64_t)idx[j] * p.H) + threadIdx.x, *reinterpret_cast<const uint4*>(o.v));
         }
       }
-      if (p.dweights) {
-        const float v = warp_sum8(dot, lane);
-        if (lane < 8) dots[dflip][warp][lane] = v;
-        __syncthreads();
-        if ((int)threadIdx.x < nj) {
-          float sum = 0.f;
-          for (int w = 0; w < warps; ++w) sum += dots[dflip][w][threadIdx.x];
-          ((T*)p.dweights)[t * p.k + j0 + threadIdx.x] = from_f32<T>(p.scale * sum);
+      if (p.dweights) store_dots(dot, t, 0, 8);
+    } else if constexpr (FORM == BWD_COMBINE) {
+      if (!p.dy && !p.dweights) continue;
+      for (int j0 = 0; j0 < p.k; j0 += 8) {
+        const int nj = min(8, p.k - j0);
+        float dot[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+          const int c = threadIdx.x + i * blockDim.x;
+          if (c >= hv) continue;
+          Vec<T> v[8];
+          int32_t r[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            r[j] = j < nj ? p.inv[t * p.k + j0 + j] : 0;
+            if (j < nj && p.dweights) *reinterpret_cast<uint4*>(v[j].v) = __ldcs(reinterpret_cast<const uint4*>(y + (int64_t)r[j] * p.H) + c);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j >= nj) continue;
+            const float w = p.dy ? p.scale * to_f32(((const T*)p.weights)[t * p.k + j0 + j]) : 0.f;
+            Vec<T> o;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+              if (p.dweights) dot[j] = fmaf(ds[i][q], to_f32(v[j].v[q]), dot[j]);
+              o.v[q] = from_f32<T>(w * ds[i][q]);
+            }
+            if (p.dy) __stcs(reinterpret_cast<uint4*>((T*)p.dy + (int64_t)r[j] * p.H) + c, *reinterpret_cast<const uint4*>(o.v));
+          }
         }
-        dflip ^= 1;  // written again two rounds on, behind the __syncthreads of the round between
+        if (p.dweights) store_dots(dot, t, j0, nj);
       }
     }
   }
@@ -421,11 +466,25 @@ int launch_fwd(const NormFwd& p, bool vec, cudaStream_t stream) {
 template <typename T>
 int launch_bwd(const NormBwd& p, void* dgamma, bool vec, cudaStream_t stream) {
   const RowShape rs = vec ? row_shape(p.H / Vec<T>::N) : RowShape{0, 0};
-  const int grid = bwd_grid(p.tokens);
-  if (rs.vpt == 1) norm_bwd_kernel<T, 1><<<grid, rs.threads, 0, stream>>>(p);
-  else if (rs.vpt == 2) norm_bwd_kernel<T, 2><<<grid, rs.threads, 0, stream>>>(p);
-  else if (rs.vpt == 4) norm_bwd_kernel<T, 4><<<grid, rs.threads, 0, stream>>>(p);
-  else {
+  int grid = bwd_grid(p.tokens);
+  // as many CTAs as are resident at once: each walks several tokens and leaves one row of partial sums
+  auto resident = [&](int ctas) { return (int)(p.tokens < (int64_t)sm_count() * ctas ? p.tokens : (int64_t)sm_count() * ctas); };
+  if (rs.vpt != 0) {
+    const int form = !p.inv ? BWD_ADD : (rs.vpt == 1 && p.k == 8) ? BWD_COMBINE8 : BWD_COMBINE;
+#define MOE_NORM_BWD(VPT, FORM)                                       \
+  if (rs.vpt == VPT && form == FORM) {                                \
+    grid = resident(norm_bwd_ctas<VPT, FORM>());                      \
+    norm_bwd_kernel<T, VPT, FORM><<<grid, rs.threads, 0, stream>>>(p); \
+  }
+    MOE_NORM_BWD(1, BWD_ADD)
+    MOE_NORM_BWD(2, BWD_ADD)
+    MOE_NORM_BWD(4, BWD_ADD)
+    MOE_NORM_BWD(1, BWD_COMBINE8)
+    MOE_NORM_BWD(1, BWD_COMBINE)
+    MOE_NORM_BWD(2, BWD_COMBINE)
+    MOE_NORM_BWD(4, BWD_COMBINE)
+#undef MOE_NORM_BWD
+  } else {
     const int smem = 2 * p.H * (int)sizeof(float);
     if (smem > 48 * 1024) {
       const int st = cuda_status(cudaFuncSetAttribute(norm_bwd_generic_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
