@@ -25,9 +25,10 @@ def grouped_gemm_fp8(pairs, m_sizes: torch.Tensor, dtype: torch.dtype, transpose
     args += [None] * (8 - len(args))
     m_sizes = _lib.as_index_tensor(m_sizes)
     y = torch.empty((M, N), device=q0.device, dtype=dtype)
-    with torch.cuda.device(q0.device):
+    here, stream = _lib.launch_on(q0.device)
+    with here:
         status = _lib.load().moe_grouped_gemm_fp8(
             int(transposed), *args, _lib.ptr(m_sizes), _lib.int_code(m_sizes.dtype), _lib.ptr(y), M, N, K, E,
-            _lib.float_code(dtype), _lib.stream_ptr(q0.device))
+            _lib.float_code(dtype), stream)
     _lib.check(status, "moe_grouped_gemm_fp8")
     return y

@@ -33,20 +33,21 @@ def _gate_up(x, gate, gate_scale, up, up_scale, m_sizes, keep: bool):
     hq, hs = _codes(M, I, x.device)
     e, g = (torch.empty((M, I), device=x.device, dtype=x.dtype) if keep else None for _ in range(2))
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+    here, stream = _lib.launch_on(x.device)
+    with here:
         status = lib.moe_gate_up_silu_fp8(
             _lib.ptr(q), _lib.ptr(s), _lib.ptr(gate), _lib.ptr(gate_scale), _lib.ptr(up), _lib.ptr(up_scale), _lib.ptr(ms),
             _lib.int_code(ms.dtype), _lib.ptr(hq), _lib.ptr(hs), _lib.ptr(e), _lib.ptr(g), M, I, K, E, _lib.float_code(x.dtype),
-            _lib.stream_ptr(x.device))
+            stream)
     if status != _lib.ERR_UNSUPPORTED:
         _lib.check(status, "moe_gate_up_silu_fp8")
         return hq, hs, e, g
     # extents or types that the kernel does not cover: the products one by one
     e32 = grouped_gemm_fp8(((q, s, gate, gate_scale),), m_sizes, torch.float32)
     g32 = grouped_gemm_fp8(((q, s, up, up_scale),), m_sizes, torch.float32)
-    with torch.cuda.device(x.device):
+    with here:
         status = lib.moe_fp8_silu_quantize(_lib.ptr(e32), _lib.ptr(g32), M, I, _lib.ptr(hq), _lib.ptr(hs), _lib.ptr(e), _lib.ptr(g),
-                                           _lib.float_code(x.dtype), _lib.stream_ptr(x.device))
+                                           _lib.float_code(x.dtype), stream)
     _lib.check(status, "moe_fp8_silu_quantize")
     return hq, hs, e, g
 
@@ -58,10 +59,11 @@ def _down_bwd(dy, down, down_scale, e, g, m_sizes):
     dh = grouped_gemm_fp8(((q, s, down, down_scale),), m_sizes, torch.float32, transposed=True)
     assert e.dtype == g.dtype == dy.dtype and e.shape == g.shape == dh.shape and e.is_contiguous() and g.is_contiguous()
     (deq, des), (dgq, dgs) = _codes(M, I, dy.device), _codes(M, I, dy.device)
-    with torch.cuda.device(dy.device):
+    here, stream = _lib.launch_on(dy.device)
+    with here:
         status = _lib.load().moe_fp8_silu_bwd_quantize(_lib.ptr(dh), _lib.ptr(e), _lib.ptr(g), M, I, _lib.ptr(deq), _lib.ptr(des),
                                                        _lib.ptr(dgq), _lib.ptr(dgs), _lib.float_code(dy.dtype),
-                                                       _lib.stream_ptr(dy.device))
+                                                       stream)
     _lib.check(status, "moe_fp8_silu_bwd_quantize")
     return deq, des, dgq, dgs
 

@@ -18,10 +18,11 @@ def _forward(y, inv_sort_idx, weights, residual, gamma, eps: float, scale: float
     total = torch.empty((T, H), device=y.device, dtype=y.dtype)
     normed = torch.empty_like(total)
     rstd = torch.empty(T, device=y.device, dtype=torch.float32) if want_rstd else None
-    with torch.cuda.device(y.device):
+    here, stream = _lib.launch_on(y.device)
+    with here:
         status = _lib.load().moe_combine_add_rms_norm(
             _lib.ptr(y), _lib.ptr(inv_sort_idx), _lib.ptr(weights), _lib.ptr(residual), _lib.ptr(gamma), scale, eps,
-            _lib.ptr(total), _lib.ptr(normed), _lib.ptr(rstd), T, k, H, _lib.float_code(y.dtype), _lib.stream_ptr(y.device))
+            _lib.ptr(total), _lib.ptr(normed), _lib.ptr(rstd), T, k, H, _lib.float_code(y.dtype), stream)
     _lib.check(status, "moe_combine_add_rms_norm")
     return normed, total, rstd
 
@@ -67,12 +68,13 @@ class CombineAddRmsNorm(torch.autograd.Function):
         dy, dw, dr, dg = out(want_y, *ctx.y_shape), out(want_w, T, k), out(want_r, T, H), out(want_g, H)
         lib = _lib.load()
         nbytes = lib.moe_combine_add_rms_norm_bwd_ws_bytes(T, H) if want_g else 0
-        with torch.cuda.device(total.device):
+        here, stream = _lib.launch_on(total.device)
+        with here:
             ws = torch.empty(nbytes, device=total.device, dtype=torch.uint8) if nbytes else None
             status = lib.moe_combine_add_rms_norm_bwd(
                 _lib.ptr(dnormed), _lib.ptr(dtotal), _lib.ptr(total), _lib.ptr(rstd), _lib.ptr(gamma), _lib.ptr(y),
                 _lib.ptr(inv_sort_idx), _lib.ptr(weights), ctx.scale, _lib.ptr(dr), _lib.ptr(dy), _lib.ptr(dw), _lib.ptr(dg),
-                T, k, H, _lib.float_code(total.dtype), _lib.ptr(ws), nbytes, _lib.stream_ptr(total.device))
+                T, k, H, _lib.float_code(total.dtype), _lib.ptr(ws), nbytes, stream)
         _lib.check(status, "moe_combine_add_rms_norm_bwd")
         return dy, None, dw, dr, dg, None, None
 

@@ -19,7 +19,9 @@ from torch.autograd import forward_ad
 from . import _lib
 from .functional import moe_fused_linear
 from .kernels.fused_mlp import gate_up_silu, gate_up_silu_forward
+from .kernels.fused_mlp_fp8 import moe_mlp_fp8
 from .kernels.indexing import get_expert_counts_and_idx
+from .kernels.norm import add_rms_norm, combine_add_rms_norm
 from .kernels.routing import combine, gather_rows, softmax_topk_autograd
 
 
@@ -129,6 +131,41 @@ def moe_block_forward(hidden_states: torch.Tensor, gate_weight: torch.Tensor, ga
     y = moe_fused_linear(h, down_proj, m_sizes)
     out = combine(y, sort_idx, inv_sort_idx, routing_weights)
     return out.view(B, S, H), router_logits
+
+
+def moe_layer_forward(hidden_states: torch.Tensor, residual: Optional[torch.Tensor], norm_weight: torch.Tensor,
+                      gate_weight: torch.Tensor, projections, num_selected: int, next_norm_weight: torch.Tensor,
+                      norm_topk_prob: bool = True, eps: float = 1e-6, scale: float = 1.0):
+    """The sparse half of a decoder layer with what stands around it, between two residual streams:
+
+        stream = residual + hidden_states             n = rms_norm(stream) * norm_weight
+        out = stream + scale * block(n)               normed = rms_norm(out) * next_norm_weight
+
+    hidden_states (B, S, H): the attention's output, or the embeddings with `residual` None; residual (B, S, H); gate_weight (E, H).
+    `projections`: (gate, up, down) in the type of the hidden states, shaped as in `moe_block_forward`, or
+    (gate, gate_scale, up, up_scale, down, down_scale) in 8 bits as in `moe_mlp_fp8`.  Returns (normed, out, router_logits): what the
+    next layer's attention reads, the stream it adds to, and the (B*S, E) logits.  Differentiable once (the 8-bit weights
+    are frozen).
+
+    The layer around the block is that of transformers; the block is the reference's
+    (qwen3_moe_fused/modular_qwen3_moe_fused.py:79-118)."""
+    assert len(projections) in (3, 6), "gate, up, down, each followed by its scales if they are in 8 bits"
+    B, S, H = hidden_states.shape
+    T, E, k = B * S, gate_weight.shape[0], num_selected
+    n, stream = add_rms_norm(hidden_states, residual, norm_weight, eps)
+    n = n.view(T, H)
+    router_logits = torch.nn.functional.linear(n, gate_weight)
+    routing_weights, selected = route(router_logits, k, norm_topk_prob, n.dtype)
+    m_sizes, sort_idx, inv_sort_idx = get_expert_counts_and_idx(selected.view(T * k), E)
+    rows = gather_rows(n, sort_idx, inv_sort_idx, k)
+    if len(projections) == 6:
+        y = moe_mlp_fp8(rows, *projections, m_sizes)
+    else:
+        gate_proj, up_proj, down_proj = projections
+        infer = not torch.is_grad_enabled() and not _has_tangent(rows, gate_proj, up_proj, down_proj)
+        y = moe_fused_linear((gate_up_silu_forward if infer else gate_up_silu)(rows, gate_proj, up_proj, m_sizes), down_proj, m_sizes)
+    normed, out = combine_add_rms_norm(y, sort_idx, inv_sort_idx, routing_weights, stream, next_norm_weight, eps, scale)
+    return normed, out, router_logits
 
 
 def fused_sparse_moe_block_forward(self, hidden_states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:

@@ -67,8 +67,9 @@ def quantize_fp8_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     M, K = x.shape
     q = torch.empty((M, K), device=x.device, dtype=FP8)
     s = empty_scales(M, K, x.device)
-    with torch.cuda.device(x.device):
+    here, stream = _lib.launch_on(x.device)
+    with here:
         status = _lib.load().moe_fp8_quantize_rows(_lib.ptr(x), _lib.float_code(x.dtype), M, K, _lib.ptr(q), _lib.ptr(s),
-                                                   _lib.stream_ptr(x.device))
+                                                   stream)
     _lib.check(status, "moe_fp8_quantize_rows")
     return q, s
