@@ -89,15 +89,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
-// mbar_wait for barriers that are met every few hundred cycles: the clock that bounds the wait takes longer to read than such a
-// wait lasts, so it is read only after a number of tries.
-__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int code) {
-#pragma unroll 1
-  for (int i = 0; i < 64; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity, abort_flag, code);
-}
-
 // For what has to be waited for even after another role aborted (a copy on its way to this CTA's shared memory): the time
 // limit is the only reason to give up.
 __device__ __forceinline__ bool mbar_wait_through(uint64_t* bar, uint32_t parity) {
@@ -169,44 +160,11 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
-// 32 lanes x 16 consecutive fp32 columns.
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16]) {
-#define MOE_R4(i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : MOE_R4(0), MOE_R4(4), MOE_R4(8), MOE_R4(12)::"memory");
-#undef MOE_R4
-}
-// 32 lanes x 64 consecutive fp32 columns.
-__device__ __forceinline__ void tmem_ld_32x64(uint32_t taddr, uint32_t (&r)[64]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
-        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
-        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
-        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
-        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
-      : "memory");
-}
 // Waits for the loads, and no use of the loaded values can be moved in front of it.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[32]) {
 #define MOE_R4(i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : MOE_R4(0), MOE_R4(4), MOE_R4(8), MOE_R4(12), MOE_R4(16), MOE_R4(20), MOE_R4(24), MOE_R4(28)::"memory");
-#undef MOE_R4
-}
-// Waits for the loads, and no use of the loaded values can be moved in front of it.
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[64]) {
-#define MOE_R4(i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : MOE_R4(0), MOE_R4(4), MOE_R4(8), MOE_R4(12), MOE_R4(16), MOE_R4(20), MOE_R4(24), MOE_R4(28), MOE_R4(32), MOE_R4(36), MOE_R4(40), MOE_R4(44), MOE_R4(48), MOE_R4(52), MOE_R4(56), MOE_R4(60)::"memory");
 #undef MOE_R4
 }
 
@@ -263,6 +221,13 @@ __device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_add
 // have been read).  A releasing arrival waits for the thread's loads in flight.
 __device__ __forceinline__ void mbar_arrive_relaxed_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// ... by lane 0 of a warp, without a branch
+__device__ __forceinline__ void arrive_lane0(uint32_t cluster_addr, int lane) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}"
+      ::"r"(cluster_addr), "r"(lane) : "memory");
 }
 // The same for writes to this CTA's own shared memory alone (sync_restrict): it does not wait for what the thread has under
 // way in global memory.

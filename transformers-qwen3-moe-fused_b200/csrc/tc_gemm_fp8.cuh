@@ -9,14 +9,19 @@
 // contraction (one stage: 128 rows x 128 bytes of either operand in each CTA) is a sum of its own in TMEM, and 8 epilogue
 // warps add it to fp32 sums in registers with its factor, acc += s ws * block.  A thread owns one token and 128 columns, one
 // block of weight rows: its factor is one number for all of them, and nothing crosses threads.  Two accumulators of 256
-// columns alternate, so the addition of one block runs beside the MMAs of the next: 512 cycles of MMA, 256 of TMEM loads,
-// 285 of packed FMAs on each quarter of the SM.
-// (With weight rows as accumulator rows the factor changes from column to column: in the fragment shape 16x256b, where a thread
-// needs few of them, TMEM loads run at half the rate (535 cycles for 256 columns, measured, against 260 in the shape
-// 32x32b), and forward / dX at 65536 rows, 2048 -> 1536, took 401 / 424 us.)
+// columns alternate, so the addition of one block runs beside the MMAs of the next.
+// (With weight rows as accumulator rows the factor changes from column to column.  In the fragment shape 16x256b, where a thread
+// needs few of them, TMEM loads run at half the rate: 535 cycles for 256 columns against 260 in the shape 32x32b.  Forward /
+// dX at 65536 rows, 2048 -> 1536: 401 / 424 us, against 309 / 318 us here.)
 //
-// The price is that a tile costs 256 rows of MMAs whatever it holds; groups of few rows are bound by their weights, and warps
-// without rows skip the additions.
+// What bounds it: the additions, not the MMAs.  With the additions left out a block takes 515 cycles, what the MMAs need at the
+// 8-bit peak, and the launch 220 us; with them 1100.  They are 256 cycles of TMEM loads and 285 of FMAs on each quarter of the
+// SM, but 128 sums, 32 loaded values and the addresses leave the compiler no registers to overlap the two (half the sums:
+// 240 us).  Narrower tiles (192 columns, 96 or 64 sums), 16 warps, four accumulators of 128 columns, scales that come by TMA, and
+// loads of 64 columns were no faster: 310 to 390 us.
+//
+// The price of tokens as rows is that a tile costs 256 rows of MMAs whatever it holds; groups of few rows are bound by their
+// weights, and warps without rows skip the additions.
 #pragma once
 
 namespace moe {
@@ -30,7 +35,7 @@ constexpr int F8_STAGE_BYTES = 2 * F8_HALF_BYTES;
 constexpr int F8_STAGES = 5;
 constexpr int F8_READERS = 5;          // of the pair's tile ring: 2 producers, 2 tile warps, the MMA thread
 constexpr int F8_TILES = 2;            // decoded tiles on their way to the epilogue warps
-constexpr int F8_EPI_REGS = 208, F8_OTHER_REGS = 88;
+constexpr int F8_EPI_REGS = 192, F8_OTHER_REGS = 120;
 static_assert(256 * F8_EPI_REGS + 128 * F8_OTHER_REGS <= F8_THREADS * 168, "shares of the registers that the CTA is launched with");
 
 struct Fp8Maps {
@@ -287,32 +292,25 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
     struct Raw { float s, w0, w1; };
     const float* sp = p.s[0];
     const float* wp = p.ws[0];
-    int fetched = 0;
-    auto start = [&](const int4& t) {
-      if (t.x < 0) return;
+    const int last = p.kb - 1;
+    auto start = [&](const int4& t, int seg) {
       const int nb = GATE_UP ? t.z / 128 : min(t.z / 128 + wg, (p.N - 1) / 128);
-      sp = p.s[0] + min(t.y + (int)rank * 128 + row, t.w - 1);
-      wp = p.ws[0] + t.x * p.ws_e + (int64_t)nb * p.ws_n;
-      fetched = 0;
+      sp = p.s[seg] + min(t.y + (int)rank * 128 + row, t.w - 1);
+      wp = p.ws[seg] + t.x * p.ws_e + (int64_t)nb * p.ws_n;
     };
-    auto fetch = [&]() {
-      Raw r = {0.f, 0.f, 0.f};
-      if (fetched < steps) {
-        r.s = __ldg(sp);
-        r.w0 = __ldg(wp);
-        if (GATE_UP) r.w1 = __ldg(wp + (p.ws[1] - p.ws[0]));
-        sp += p.pitch;
-        wp += p.ws_k;
-        if (++fetched == p.kb && !GATE_UP) {  // on to the second operand pair
-          sp += (p.s[1] - p.s[0]) - p.kb * p.pitch;
-          wp += (p.ws[1] - p.ws[0]) - (int64_t)p.kb * p.ws_k;
-        }
-      }
+    auto fetch = [&](int b) {
+      Raw r;
+      const uint32_t kb = (uint32_t)min(b, last);  // (past the last block: the last one again, not used)
+      r.s = __ldg(sp + (uint64_t)kb * (uint32_t)p.pitch);
+      r.w0 = __ldg(wp + kb * (uint32_t)p.ws_k);
+      r.w1 = GATE_UP ? __ldg(wp + (p.ws[1] - p.ws[0]) + kb * (uint32_t)p.ws_k) : 0.f;
       return r;
     };
     int4 info = take();
-    start(info);
-    Raw r0 = fetch(), r1 = fetch();
+    if (info.x >= 0) start(info, 0);
+    Raw r0 = {}, r1 = {};
+    if (info.x >= 0) { r0 = fetch(0); r1 = fetch(1); }
+    bool ready = false;  // the next block's sums were seen to be there while this one was added
     while (true) {
       const bool leave = __any_sync(0xffffffffu, info.x < 0);
       if constexpr (GATE_UP) {  // the two warps that share tokens leave together
@@ -327,45 +325,63 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
       uint64_t acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = 0;
-      auto add_block = [&](const Raw& r) {
+      // The loads of the factors and the test for the next block stand where the thread would wait for TMEM or has additions to
+      // issue.
+      auto add_block = [&](Raw& r, int ahead) {
         const uint32_t buf = it & 1;
-        ok = ok && mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
+        if (!ready) ok = ok && mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
         tc_fence_after_sync();
         ++it;
-        if (live) {
-          const uint32_t taddr = taddr0 + buf * 256;
+        const uint32_t taddr = taddr0 + buf * 256;
+        uint32_t f0, f1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           uint32_t v[32];
-          const uint32_t f0 = __float_as_uint(r.s * r.w0), f1 = GATE_UP ? __float_as_uint(r.s * r.w1) : f0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            tmem_ld_32x32(taddr + i * 32, v);
-            tmem_ld_wait(v);
-            if (i == 3) {
-              tc_fence_before_sync();
-              if (lane == 0) mbar_arrive_relaxed_cluster(tmem_free_leader0 + buf * 8);  // (the wait above was the whole warp's)
-            }
-            const uint64_t ff = i < 2 ? pack_f32x2(f0, f0) : pack_f32x2(f1, f1);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[i * 16 + j] = fma_f32x2(pack_f32x2(v[2 * j], v[2 * j + 1]), ff, acc[i * 16 + j]);
+          tmem_ld_32x32(taddr + i * 32, v);
+          if (i == 0) {
+            f0 = __float_as_uint(r.s * r.w0);
+            f1 = GATE_UP ? __float_as_uint(r.s * r.w1) : f0;
+            r = fetch(ahead);
           }
-        } else {
-          if (lane == 0) mbar_arrive_relaxed_cluster(tmem_free_leader0 + buf * 8);
+          tmem_ld_wait(v);
+          if (i == 3) {
+            tc_fence_before_sync();
+            arrive_lane0(tmem_free_leader0 + buf * 8, lane);  // (the wait above was the whole warp's)
+            ready = mbar_test(&ctl->tmem_full[it & 1], (it >> 1) & 1);
+          }
+          const uint64_t ff = i < 2 ? pack_f32x2(f0, f0) : pack_f32x2(f1, f1);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[i * 16 + j] = fma_f32x2(pack_f32x2(v[2 * j], v[2 * j + 1]), ff, acc[i * 16 + j]);
         }
       };
+      if (live) {
+        for (int seg = 0; seg < p.n_seg; ++seg) {
+          if (seg > 0) {
+            start(info, 1);
+            r0 = fetch(0);
+            r1 = fetch(1);
+          }
 #pragma unroll 1
-      for (int b = 0; b < steps; b += 2) {
-        const Raw c0 = r0, c1 = r1;
-        r0 = fetch();
-        add_block(c0);
-        if (b + 1 < steps) {
-          r1 = fetch();
-          add_block(c1);
+          for (int b = 0; b < p.kb; b += 2) {
+            add_block(r0, b + 2);
+            if (b + 1 < p.kb) add_block(r1, b + 3);
+          }
         }
+      } else {
+        for (int b = 0; b < steps; ++b, ++it) {
+          ok = ok && mbar_wait(&ctl->tmem_full[it & 1], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
+          tc_fence_after_sync();
+          __syncwarp();
+          arrive_lane0(tmem_free_leader0 + (it & 1) * 8, lane);
+        }
+        ready = false;
       }
       info = take();
-      start(info);
-      r0 = fetch();
-      r1 = fetch();
+      if (info.x >= 0) {
+        start(info, 0);
+        r0 = fetch(0);
+        r1 = fetch(1);
+      }
       if constexpr (!GATE_UP) {
         if (!live) continue;
         const int n0 = t_n0 + wg * 128;  // first column
