@@ -59,3 +59,13 @@ def test_weight_codes():
     # half a step: 2^-4 of the value (the quotient is rounded once more, 2^-24) or 2^-10 of the scale
     full = s.repeat_interleave(128, 1)[:, :130].repeat_interleave(128, 2)[:, :, :257]
     assert bool(((dequantize_fp8(codes, s) - w).abs() <= w.abs() * 2.0 ** -4 * (1 + 2.0 ** -20) + full * 2.0 ** -10).all())
+
+
+def test_extents_past_an_int_are_refused(lib):
+    big = (1 << 24) + 1
+    none8 = [None] * 8
+    for N, K in ((big, 8), (8, big), (2 ** 31 - 1, 8), (8, 2 ** 31 - 1)):
+        assert lib.moe_grouped_gemm_fp8(0, *none8, None, 3, None, 4, N, K, 2, 1, None) == -2
+        assert lib.moe_gate_up_silu_fp8(*[None] * 7, 3, *[None] * 4, 4, N, K, 2, 1, None) == -2
+    assert lib.moe_fp8_quantize_rows(None, 1, 4, big, None, None, None) == -2
+    assert lib.moe_fp8_quantize_rows(None, 1, 2 ** 31, 8, None, None, None) == -2

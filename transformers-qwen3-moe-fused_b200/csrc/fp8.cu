@@ -280,7 +280,10 @@ dim3 quantize_grid(int64_t M, int K, int unroll) {
 
 bool aligned8(const void* p) { return ((uintptr_t)p & 7) == 0; }
 
-bool rows_ok(int64_t M, int K) { return M >= 0 && M <= 0x7fffffffLL && K >= 1 && K <= 1 << 24; }  // (K: the grid's second extent)
+constexpr int MAX_EXTENT = 1 << 24;  // of N and K: the grids' second extent, and tile and block ends fit in an int
+
+bool rows_ok(int64_t M, int K) { return M >= 0 && M <= 0x7fffffffLL && K >= 1 && K <= MAX_EXTENT; }
+bool product_ok(int64_t M, int N, int K) { return M <= 0x7fffffffLL - 1024 && rows_ok(M, K) && N >= 1 && N <= MAX_EXTENT; }
 
 }  // namespace
 }  // namespace moe
@@ -342,7 +345,7 @@ MOE_API int moe_gate_up_silu_fp8(const void* q, const float* s, const void* w_ga
                                  const float* ws_up, const void* m_sizes, int msd, void* hq, float* hs, void* keep_e,
                                  void* keep_g, int64_t M, int I, int K, int E, int dtype, void* stream) {
   if (!is_float_dtype(dtype) || !is_int_dtype(msd)) return MOE_ERR_DTYPE;
-  if (M < 0 || M > 0x7fffffffLL - 1024 || I < 1 || K < 1 || E < 1) return MOE_ERR_SHAPE;
+  if (!product_ok(M, I, K) || E < 1) return MOE_ERR_SHAPE;
   if (M == 0) return MOE_OK;
   if (!q || !s || !w_gate || !ws_gate || !w_up || !ws_up || !m_sizes || !hq || !hs || !keep_e != !keep_g) return MOE_ERR_NULL;
   const int path = moe_get_gemm_path();
@@ -358,7 +361,7 @@ MOE_API int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const
                                  int64_t M, int N, int K, int E, int dtype_out, void* stream_) {
   cudaStream_t stream = (cudaStream_t)stream_;
   if (!is_float_dtype(dtype_out) || !is_int_dtype(msd)) return MOE_ERR_DTYPE;
-  if ((which != 0 && which != 1) || M < 0 || M > 0x7fffffffLL - 1024 || N < 1 || K < 1 || E < 1 || E > 65535) return MOE_ERR_SHAPE;
+  if ((which != 0 && which != 1) || !product_ok(M, N, K) || E < 1 || E > 65535) return MOE_ERR_SHAPE;
   if (M == 0) return MOE_OK;
   if (!q || !s || !w || !ws || !m_sizes || !y || (q2 && (!s2 || !w2 || !ws2))) return MOE_ERR_NULL;
   const int ms64 = msd == MOE_I64;
