@@ -57,7 +57,9 @@ def _down_bwd(dy, down, down_scale, e, g, m_sizes):
     q, s = quantize_fp8_rows(dy)
     M, I = e.shape
     dh = grouped_gemm_fp8(((q, s, down, down_scale),), m_sizes, torch.float32, transposed=True)
+    # (hooks on saved tensors may have given back another type, device or layout)
     assert e.dtype == g.dtype == dy.dtype and e.shape == g.shape == dh.shape and e.is_contiguous() and g.is_contiguous()
+    assert e.device == g.device == dy.device
     (deq, des), (dgq, dgs) = _codes(M, I, dy.device), _codes(M, I, dy.device)
     here, stream = _lib.launch_on(dy.device)
     with here:
