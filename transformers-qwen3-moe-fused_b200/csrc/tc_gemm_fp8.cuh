@@ -20,8 +20,8 @@
 // 240 us).  Narrower tiles (192 columns, 96 or 64 sums), 16 warps, four accumulators of 128 columns, scales that come by TMA, and
 // loads of 64 columns were no faster: 310 to 390 us.
 //
-// The price of tokens as rows is that a tile costs 256 rows of MMAs whatever it holds; groups of few rows are bound by their
-// weights, and warps without rows skip the additions.
+// The price of tokens as rows is that a tile costs 256 rows of MMAs whatever it holds (warps without rows skip the additions);
+// groups of few rows have a kernel of their own, thin_fp8_kernel.
 #pragma once
 
 namespace moe {
