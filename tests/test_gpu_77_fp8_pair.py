@@ -1,0 +1,41 @@
+"""The CTA-pair kernel of the 8-bit products, forced on groups of any size."""
+import pytest
+import torch
+
+from . import test_gpu_73_fp8 as products
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def pairs():
+    from qwen3_moe_fused import _lib
+
+    prev = _lib.set_gemm_path(_lib.PATH_TC)
+    yield "pairs"
+    _lib.set_gemm_path(prev)
+    torch.cuda.synchronize()
+    assert _lib.read_error_flag() == 0
+
+
+@pytest.mark.parametrize("K,N", [(2048, 1536), (128, 512), (384, 208)])
+def test_the_same_bits_in_every_run(cuda, pairs, K, N):
+    """Accumulators are handed back and overwritten a few hundred cycles after they are read: a reading that came late would show."""
+    from qwen3_moe_fused.quantize.linear8bit import moe_fused_linear_fp8
+
+    gen = products.gen_for(cuda, K)
+    codes, s = products.fp8_weight(16, N, K, gen, cuda)
+    sizes = torch.bincount((torch.rand(9001, generator=gen, device=cuda) ** 2 * 16).long(), minlength=16)
+    x = torch.randn(9001, K, generator=gen, device=cuda).to(torch.bfloat16).requires_grad_()
+    dy = torch.randn(9001, N, generator=gen, device=cuda).to(torch.bfloat16)
+
+    def run():
+        y = moe_fused_linear_fp8(x, codes, s, sizes)
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    want = run()
+    differ = torch.zeros((), device=cuda, dtype=torch.int64)
+    for _ in range(200):
+        for a, b in zip(run(), want):
+            differ += (a != b).sum()
+    assert differ.item() == 0

@@ -330,6 +330,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
       auto add_block = [&](Raw& r, int ahead) {
         const uint32_t buf = it & 1;
         if (!ready) ok = ok && mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
+        __syncwarp();  // (each lane tests and waits for itself; the TMEM loads, and the arrival behind them, are the whole warp's)
         tc_fence_after_sync();
         ++it;
         const uint32_t taddr = taddr0 + buf * 256;
