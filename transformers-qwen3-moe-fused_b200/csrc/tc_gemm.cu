@@ -335,7 +335,8 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant_
       const bool row_ok = grow < row_start[e + 1] && grow < p.M;
       const uint32_t acc = acc_it & 1;
       const uint32_t acc_ph = (acc_it >> 1) & 1;
-      if (!mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, W_TMEM_FULL)) { ok = false; break; }
+      // (voted on: lanes whose looks at the barrier differed come back together for the TMEM loads)
+      if (!__all_sync(0xffffffffu, mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, W_TMEM_FULL))) { ok = false; break; }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + acc * ACC_STRIDE + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
@@ -511,7 +512,8 @@ tc_fwd_nf4_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_const
       const bool row_ok = grow < row_start[e + 1] && grow < p.M;
       const uint32_t acc = acc_it & 1;
       const uint32_t acc_ph = (acc_it >> 1) & 1;
-      if (!mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, W_TMEM_FULL)) { ok = false; break; }
+      // (voted on: lanes whose looks at the barrier differed come back together for the TMEM loads)
+      if (!__all_sync(0xffffffffu, mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, W_TMEM_FULL))) { ok = false; break; }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + acc * BN + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1

@@ -242,7 +242,8 @@ pair_fwd_nf4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_con
       const uint32_t acc_ph = (acc_it >> 1) & 1;
       const CUtensorMap* my = staged ? p.group_maps + (size_t)GM_OUT * p.E + e : nullptr;
       if (staged && epi_tid == 0 && e != last_e) { tensormap_acquire(my); last_e = e; }
-      if (!mbar_wait_cluster(&ctl->tmem_full[acc], acc_ph, abort_flag, PW_TMEM_FULL)) { ok = false; break; }
+      // the lanes come back together for the TMEM loads, and the four warps leave together
+      if (named_barrier_any(2, 128, !mbar_wait_cluster(&ctl->tmem_full[acc], acc_ph, abort_flag, PW_TMEM_FULL))) { ok = false; break; }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + acc * PAIR_TOKENS + ((uint32_t)(quarter * 32) << 16);
       if (staged) {
