@@ -277,11 +277,14 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
     uint8_t* const my_staging = staging + (warp - 4) * (2 * F8_WARP_STAGING);
     const uint32_t taddr0 = tmem_base + ((uint32_t)(quarter * 32) << 16) + wg * 128;
     uint32_t it = 0, n_tile = 0;
-    bool ok = true;  // a warp whose wait was abandoned goes on without waiting to the end of the tile
+    // A warp with an abandoned wait goes on to the end of the tile without waiting, but lane 0 hands no accumulator back any more
+    // (other warps, the other CTA's too, may still have to read it), and no warp of the CTA stores sums.  `sign` is the lane, or 32
+    // behind an abandoned wait.
+    int sign = lane;
     auto take = [&]() {
       const uint32_t slot = n_tile % F8_TILES;
-      ok = ok && mbar_wait(&ctl->tile_full[slot], (n_tile / F8_TILES) & 1, abort_flag, FW_TILE_FULL);
-      const int4 info = ok ? ctl->tiles[slot] : make_int4(-1, 0, 0, 0);
+      const bool there = sign != 32 && mbar_wait(&ctl->tile_full[slot], (n_tile / F8_TILES) & 1, abort_flag, FW_TILE_FULL);
+      const int4 info = there ? ctl->tiles[slot] : make_int4(-1, 0, 0, 0);
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl->tile_empty[slot]);
       ++n_tile;
@@ -329,7 +332,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
       // issue.
       auto add_block = [&](Raw& r, int ahead) {
         const uint32_t buf = it & 1;
-        if (!ready) ok = ok && mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
+        if (!ready && (sign == 32 || !mbar_wait(&ctl->tmem_full[buf], (it >> 1) & 1, abort_flag, PW_TMEM_FULL))) sign = 32;
         __syncwarp();  // (each lane tests and waits for itself; the TMEM loads, and the arrival behind them, are the whole warp's)
         tc_fence_after_sync();
         ++it;
@@ -347,7 +350,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
           tmem_ld_wait(v);
           if (i == 3) {
             tc_fence_before_sync();
-            arrive_lane0(tmem_free_leader0 + buf * 8, lane);  // (the wait above was the whole warp's)
+            arrive_lane0(tmem_free_leader0 + buf * 8, sign);  // (the wait above was the whole warp's)
             ready = mbar_test(&ctl->tmem_full[it & 1], (it >> 1) & 1);
           }
           const uint64_t ff = i < 2 ? pack_f32x2(f0, f0) : pack_f32x2(f1, f1);
@@ -370,13 +373,14 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         }
       } else {
         for (int b = 0; b < steps; ++b, ++it) {
-          ok = ok && mbar_wait(&ctl->tmem_full[it & 1], (it >> 1) & 1, abort_flag, PW_TMEM_FULL);
+          if (sign == 32 || !mbar_wait(&ctl->tmem_full[it & 1], (it >> 1) & 1, abort_flag, PW_TMEM_FULL)) sign = 32;
           tc_fence_after_sync();
           __syncwarp();
-          arrive_lane0(tmem_free_leader0 + (it & 1) * 8, lane);
+          arrive_lane0(tmem_free_leader0 + (it & 1) * 8, sign);
         }
         ready = false;
       }
+      const bool whole = !__any_sync(0xffffffffu, *abort_flag != 0);  // nobody here gave up: every block is in the sums
       info = take();
       if (info.x >= 0) {
         start(info, 0);
@@ -384,7 +388,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         r1 = fetch(1);
       }
       if constexpr (!GATE_UP) {
-        if (!live) continue;
+        if (!live || !whole) continue;
         const int n0 = t_n0 + wg * 128;  // first column
         if (p.dtype_out == MOE_F32) {
           float* out = reinterpret_cast<float*>(p.out) + (int64_t)(tok0 + lane) * p.N + n0;
@@ -436,7 +440,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
       } else {
         if (!live) continue;  // (the same for the two warps that share the tokens)
         const int tok = tok0 + lane, f0 = t_n0 + wg * 64;
-        const bool mine = lane < rows;
+        bool mine = lane < rows && whole;
         if (p.keep_e != nullptr && mine) {
           const bool is_bf16 = p.dtype_out == MOE_BF16;
 #pragma unroll
@@ -463,9 +467,11 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         }
         // the scale's other 64 features are with the other warpgroup; the next tile's words are written behind the vote above
         uint32_t* tops = reinterpret_cast<uint32_t*>(staging);
-        tops[wg * 128 + row] = top;
+        tops[wg * 128 + row] = whole ? top : 0xffffffffu;  // (above the bits of any magnitude)
         named_barrier_sync(1 + quarter, 64);
-        top = max(top, tops[(wg ^ 1) * 128 + row]);
+        const uint32_t other = tops[(wg ^ 1) * 128 + row];
+        mine = mine && other != 0xffffffffu;
+        top = max(top, other);
         float inv;
         const float scale = fp8_block_scale(top, inv);
         if (mine) {
