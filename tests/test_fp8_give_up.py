@@ -1,8 +1,8 @@
 """The CTA-pair kernel of the 8-bit products (csrc/tc_gemm_fp8.cuh) when a wait is abandoned, as a model under random schedules: two
 producers, the MMA thread, epilogue warps of both CTAs, loads and MMAs that end in their own time.  One role gives up at a random
-wait, which stops its CTA; the other CTA's waits run out when nothing moves any more.  Nothing that is stored lacks a block or
-holds another one's sums.  Without the rules that the kernel follows (no hand-back and no stores behind an abandoned wait) the model
-finds such stores."""
+wait, which stops its CTA; the other CTA's waits run out at any time behind that, at the latest when nothing moves any more.
+Nothing that is stored lacks a block or holds another one's sums.  Without the rules that the kernel follows (no hand-back and no
+stores behind an abandoned wait) the model finds such stores."""
 import random
 import re
 
@@ -72,20 +72,20 @@ class Pair:
         count = 0
         while True:
             live = {i: w for i, w in live.items() if w != "over"}
+            if not live:
+                return
             ready = [i for i, w in live.items() if w is None or w()]
             stopped = [i for i, w in live.items() if w is not None and not w() and self.abort[self.roles[i][0]]]
             events = [("role", i, True) for i in ready] + [("role", i, False) for i in stopped] + \
                 [("land", x, 0) for x in self.loading] + ([("commit", 0, 0)] if self.consumed < self.started else [])
             count += 1
-            if count == give_up_at and live:
+            if count == give_up_at or any(self.abort) and self.rng.random() < 0.05:  # (further limits at any time)
                 waiting = [i for i, w in live.items() if w is not None]
                 if waiting:
                     i = self.rng.choice(waiting)
                     self.abort[self.roles[i][0]] = True
                     events = [("role", i, False)]
             if not events:
-                if not live:
-                    return
                 i = self.rng.choice(list(live))  # a wait that ran into its limit
                 self.abort[self.roles[i][0]] = True
                 events = [("role", i, False)]
@@ -133,3 +133,11 @@ def test_the_kernel_follows_the_rules(rule):
     """The places where an epilogue warp hands back an accumulator or stores."""
     assert len(re.findall(rule, SOURCE)) == 1
     assert len(re.findall(r"arrive_lane0\(tmem_free", SOURCE)) == 2
+
+
+def test_the_kernel_for_few_rows_hands_nothing_back_either():
+    """The same rule in tc_gemm_fp8_thin.cuh, whose warps leave ahead of their stores."""
+    thin = (PKG_ROOT / "csrc" / "tc_gemm_fp8_thin.cuh").read_text()
+    signs = [line.split("//")[0].strip() for line in thin.splitlines() if "mbar_arrive(&ctl->tmem_free" in line]
+    assert signs == ["if (lane == 0 && ok) mbar_arrive(&ctl->tmem_free[s]);"]
+    assert re.search(r"const bool leave = __any_sync\(0xffffffffu, !ok\);\s+if constexpr \(!GATE_UP\) \{\s+if \(leave\) break;", thin)

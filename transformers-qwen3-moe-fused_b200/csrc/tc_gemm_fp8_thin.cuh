@@ -219,7 +219,7 @@ thin_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         }
         tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->tmem_free[s]);
+        if (lane == 0 && ok) mbar_arrive(&ctl->tmem_free[s]);  // (not behind an abandoned wait: the other warps may still have to read it)
         ++it;
       }
     };
