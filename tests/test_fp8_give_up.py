@@ -1,8 +1,9 @@
 """The CTA-pair kernel of the 8-bit products (csrc/tc_gemm_fp8.cuh) when a wait is abandoned, as a model under random schedules: two
 producers, the MMA thread, epilogue warps of both CTAs, loads and MMAs that end in their own time.  One role gives up at a random
 wait, which stops its CTA; the other CTA's waits run out at any time behind that, at the latest when nothing moves any more.
-Nothing that is stored lacks a block or holds another one's sums.  Without the rules that the kernel follows (no hand-back and no
-stores behind an abandoned wait) the model finds such stores."""
+Nothing that is stored lacks a block or holds another one's sums, and no copy or MMA is under way when the CTAs end.  Without the
+rules that the kernel follows (no hand-back and no stores behind an abandoned wait; the MMA thread waits for its last MMA, the
+leader for the stages behind it) the model finds such stores and such ends."""
 import random
 import re
 
@@ -102,6 +103,33 @@ class Pair:
                     live[x] = "over"
 
 
+    def under_way(self, drain):
+        """Copies and MMAs that are not over when both CTAs end."""
+        if drain:
+            self.consumed = self.started
+            for b in range(self.started, max(self.issued)):
+                if b < min(self.issued):
+                    self.loading = [x for x in self.loading if x[1] != b]  # full: both CTAs' copies
+                else:
+                    self.loading = []  # never full: the limit, longer than any copy takes
+        return len(self.loading) + self.started - self.consumed
+
+
+def ends(drain, runs=3000):
+    rng = random.Random(3)
+    busy = 0
+    for _ in range(runs):
+        pair = Pair(rng.randrange(1, 4), rng.randrange(1, 9), True, rng)
+        pair.run(rng.randrange(1, 150))
+        assert max(pair.issued) - pair.started <= STAGES  # the barriers' phases tell the stages apart
+        busy += pair.under_way(drain) > 0
+    return busy
+
+
+def test_nothing_is_under_way_at_the_end():
+    assert ends(True) == 0 and ends(False) > 0
+
+
 def stores(rules, runs=3000):
     rng = random.Random(1)
     bad = 0
@@ -133,6 +161,15 @@ def test_the_kernel_follows_the_rules(rule):
     """The places where an epilogue warp hands back an accumulator or stores."""
     assert len(re.findall(rule, SOURCE)) == 1
     assert len(re.findall(r"arrive_lane0\(tmem_free", SOURCE)) == 2
+
+
+def test_the_kernel_waits_for_what_is_under_way():
+    """Behind the MMA loop the drain, behind the cluster barrier the stages, ahead of freeing TMEM."""
+    places = [r"report_stages\(\(int\)rank, loaded\);", r"report_stages\(2, \(int\)it\);\s+umma_commit_pair\(&ctl->drain, 1\);[^\n]*\n\s+"
+              r"mbar_wait_through\(&ctl->drain, 0\);", r"cluster_sync_all\(\);  // nobody frees", r"if \(done\[0\] != done\[2\]",
+              r"tmem_dealloc_pair\("]
+    at = [re.search(place, SOURCE).start() for place in places]
+    assert at == sorted(at)
 
 
 def test_the_kernel_for_few_rows_hands_nothing_back_either():

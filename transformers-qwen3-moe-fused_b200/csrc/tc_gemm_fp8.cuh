@@ -77,6 +77,8 @@ struct Fp8Control {
   uint64_t cancel_bar;
   alignas(16) uint4 cancel_response;
   int4 tiles[F8_TILES];           // expert (-1: no more tiles), first token, first column, first row past the expert
+  uint64_t drain;                 // the MMA thread's last MMAs
+  int stages_done[3];             // loaded by the leader's producer, by the other CTA's, multiplied; the same in both CTAs
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -128,6 +130,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
     for (int q = 0; q < F8_TILES; ++q) { mbar_init(&ctl->tile_full[q], 1); mbar_init(&ctl->tile_empty[q], 8); }
     Feed::init(&ctl->sched);
     mbar_init(&ctl->cancel_bar, 1);
+    mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&maps.w[0]);
@@ -146,6 +149,10 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
   const int n_tiles = (p.N + TILE_N - 1) / TILE_N;
   const int64_t total_tiles = (int64_t)tt_start[p.E] * n_tiles;
   const int steps = p.kb * p.n_seg;  // stages of a tile
+
+  auto report_stages = [&](int who, int n) {
+    for (uint32_t c = 0; c < 2; ++c) st_shared_cluster_u32(map_to_cta(smem_u32(&ctl->stages_done[who]), c), (uint32_t)n);
+  };
 
   // Within an expert the token tile varies fastest: neighbouring tiles read the same weight slice.
   auto decode = [&](int tile) {
@@ -172,7 +179,7 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         // nobody reads
         auto small_boxes = [&](int rows) { return rows > 64 ? 0 : rows <= 0 ? -1 : (rows + PAIR_SMALL_BOX - 1) / PAIR_SMALL_BOX; };
         auto box_bytes = [&](int boxes) { return boxes < 0 ? 0 : boxes == 0 ? F8_HALF_BYTES : boxes * PAIR_SMALL_BOX * F8_BK; };
-        int s = 0;
+        int s = 0, loaded = 0;
         uint32_t ph = 0;
         bool ok = true;
         while (ok) {
@@ -201,10 +208,12 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
               if (nsb == 0) tma_load_2d_pair(sa, &maps.x[i], bar, kb * F8_BK, tok);
               for (int b = 0; b < nsb; ++b)
                 tma_load_2d_pair(sa + b * (PAIR_SMALL_BOX * F8_BK), &maps.xs[i], bar, kb * F8_BK, tok + b * PAIR_SMALL_BOX);
+              ++loaded;
               if (++s == p.stages) { s = 0; ph ^= 1; }
             }
           }
         }
+        report_stages((int)rank, loaded);
       }
     } else if (warp == 1) {
       // ------------- MMA issuer (leader CTA); the same warp of the other CTA draws the tiles -------------
@@ -243,6 +252,9 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
             if (b == 0) tile = feed.take();  // the next one, while this tile's blocks are on their way
           }
         }
+        report_stages(2, (int)it);
+        umma_commit_pair(&ctl->drain, 1);  // operands and accumulators of both CTAs stay until the last MMA is over
+        mbar_wait_through(&ctl->drain, 0);
       }
     } else if (warp == 2) {
       // ---------------- tiles for the epilogue (both CTAs): taken from the pair's ring and decoded ----------------
@@ -497,6 +509,18 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
 
   tc_fence_before_sync();
   cluster_sync_all();  // nobody frees TMEM or exits while the peer may still touch this CTA
+  // A stage that was multiplied had landed.  Where somebody gave up, the ones that were loaded behind it are waited for; one that
+  // only one of the CTAs loaded does not become full, and the limit is for all of them together.
+  const int* done = ctl->stages_done;
+  if (done[0] != done[2] || done[1] != done[2]) {
+    if (leader && threadIdx.x == 0) {
+      const unsigned long long t0 = global_ns();
+      for (int i = done[2], n = max(done[0], done[1]); i < n; ++i)
+        while (!mbar_try_wait_cluster(&ctl->full[i % p.stages], (uint32_t)(i / p.stages) & 1) && global_ns() - t0 <= WAIT_LIMIT_NS) {}
+    }
+    __syncwarp();
+    cluster_sync_all();
+  }
   if (warp == 1) {
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, TMEM_COLS);
