@@ -178,3 +178,14 @@ def test_the_kernel_for_few_rows_hands_nothing_back_either():
     signs = [line.split("//")[0].strip() for line in thin.splitlines() if "mbar_arrive(&ctl->tmem_free" in line]
     assert signs == ["if (lane == 0 && ok) mbar_arrive(&ctl->tmem_free[s]);"]
     assert re.search(r"const bool leave = __any_sync\(0xffffffffu, !ok\);\s+if constexpr \(!GATE_UP\) \{\s+if \(leave\) break;", thin)
+
+
+def test_the_kernel_for_few_rows_waits_whoever_gave_up():
+    """Its producer waits for its last copies and its MMA thread for its last MMAs also where their own waits have held: whoever reads
+    them may have left."""
+    thin = (PKG_ROOT / "csrc" / "tc_gemm_fp8_thin.cuh").read_text()
+    loop = re.search(r"\n( *)for \(int i = it > STAGES \? it - STAGES : 0; i < it; \+\+i\) mbar_wait_through\(&ctl->full\[i % STAGES\], "
+                     r"\(i / STAGES\) & 1\);", thin)
+    drain = re.search(r"\n( *)umma_commit\(&ctl->drain\);[^\n]*\n( *)mbar_wait_through\(&ctl->drain, 0\);", thin)
+    role = len(re.search(r"\n( *)int it = 0;", thin).group(1))  # indented like the role's first line: under no condition of its own
+    assert [len(g) for g in (loop.group(1), *drain.groups())] == [role] * 3

@@ -32,7 +32,7 @@ struct Fp8ThinControl {
   uint64_t empty[F8T_STAGES];
   uint64_t tmem_full[F8T_STAGES];
   uint64_t tmem_free[F8T_STAGES];  // 4 warps
-  uint64_t drain;                  // MMAs of a CTA that gave up
+  uint64_t drain;                  // the last MMAs
   alignas(16) uint32_t tops[fp8_thin_rows(true)][4];  // GATE_UP: largest magnitude of a token in each warp's features
   uint32_t tmem_base;
   int abort_flag;
@@ -138,8 +138,8 @@ thin_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
           }
         }
       }
-      if (!ok)  // the copies on their way
-        for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait_through(&ctl->full[i % STAGES], (i / STAGES) & 1);
+      // the copies on their way: an MMA thread that gave up does not wait for them
+      for (int i = it > STAGES ? it - STAGES : 0; i < it; ++i) mbar_wait_through(&ctl->full[i % STAGES], (i / STAGES) & 1);
     }
   } else if (warp == 1) {
     // ------------------------------ MMA issuer ------------------------------
@@ -167,10 +167,8 @@ thin_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
           umma_commit(&ctl->tmem_full[s]);
         }
       }
-      if (!ok) {
-        umma_commit(&ctl->drain);
-        mbar_wait_through(&ctl->drain, 0);
-      }
+      umma_commit(&ctl->drain);  // an epilogue warp that gave up does not wait for the last MMAs
+      mbar_wait_through(&ctl->drain, 0);
     }
   } else {
     // ------------------------------ epilogue ------------------------------
