@@ -47,8 +47,8 @@ __device__ __forceinline__ void store_codes(const float (&v)[8], uint32_t top, u
   }
 }
 
-// A warp takes UNROLL neighbouring pairs of blocks of a row (blockIdx.y: which of them) and loads all before it works on the
-// first one.
+// A warp takes UNROLL neighbouring pairs of blocks of a row (blockIdx.x: which of them; a long row has more than the grid's
+// second extent could count) and loads all before it works on the first one.
 struct RowBlock {
   int64_t row;
   int col, kb;
@@ -56,9 +56,9 @@ struct RowBlock {
 template <int UNROLL, typename Values, typename Load, typename Work>
 __device__ __forceinline__ void for_row_blocks(int64_t M, int K, Load load, Work work) {
   const int lane = threadIdx.x & 31;
-  const int p0 = blockIdx.y * UNROLL;
-  const int64_t step = (int64_t)gridDim.x * (Q_THREADS / 32);
-  for (int64_t row = (int64_t)blockIdx.x * (Q_THREADS / 32) + (threadIdx.x >> 5); row < M; row += step) {
+  const int p0 = blockIdx.x * UNROLL;
+  const int64_t step = (int64_t)gridDim.y * (Q_THREADS / 32);
+  for (int64_t row = (int64_t)blockIdx.y * (Q_THREADS / 32) + (threadIdx.x >> 5); row < M; row += step) {
     Values v[UNROLL];
     auto at = [&](int u) { return RowBlock{row, (p0 + u) * 2 * FP8_BLOCK + lane * 8, 2 * (p0 + u) + (lane >> 4)}; };
 #pragma unroll
@@ -275,12 +275,12 @@ simt_gemm_fp8_kernel(const Fp8Pairs ops, const void* m_sizes, int ms64, T* __res
 dim3 quantize_grid(int64_t M, int K, int unroll) {
   const int64_t pairs = (K + 2 * FP8_BLOCK - 1) / (2 * FP8_BLOCK), groups = (pairs + unroll - 1) / unroll;
   const int64_t want = (M + Q_THREADS / 32 - 1) / (Q_THREADS / 32), cap = (int64_t)sm_count() * 16 / groups + 1;
-  return dim3((unsigned)(want < cap ? want : cap), (unsigned)groups);
+  return dim3((unsigned)groups, (unsigned)(want < cap ? want : cap));
 }
 
 bool aligned8(const void* p) { return ((uintptr_t)p & 7) == 0; }
 
-constexpr int MAX_EXTENT = 1 << 24;  // of N and K: the grids' second extent, and tile and block ends fit in an int
+constexpr int MAX_EXTENT = 1 << 24;  // of N and K: tile and block ends fit in an int
 
 bool rows_ok(int64_t M, int K) { return M >= 0 && M <= 0x7fffffffLL && K >= 1 && K <= MAX_EXTENT; }
 bool product_ok(int64_t M, int N, int K) { return M <= 0x7fffffffLL - 1024 && rows_ok(M, K) && N >= 1 && N <= MAX_EXTENT; }
