@@ -334,14 +334,21 @@ int moe_combine_add_rms_norm(const void* y, const int32_t* inv_sort_idx, const v
                              int H, int dtype, void* stream);
 
 /* Its gradients from those of normed and sum (dnormed, dsum: either may be NULL = zeros): dresidual (T,H), dy (rows of y),
- * dweights (T,k), dgamma (H), each NULL where it is not wanted.  sum and rstd as the forward wrote them.  dgamma needs ws of
+ * dweights (T,k), dgamma (H), each NULL where it is not wanted.  rstd as the forward wrote it.  dgamma needs ws of
  * moe_combine_add_rms_norm_bwd_ws_bytes bytes, 16-byte aligned (scratch), and is the same in every run.
+ * _bwd_inputs forms the sum again from residual, y and weights, with the forward's bits before their rounding; y is needed for
+ * every gradient but those of dsum alone.  _bwd takes the sum as the forward stored it, for callers that kept neither residual
+ * nor y: gradients carry its rounding, and are not finite where a sum left the range of dtype.
  * No counterpart in the reference, which leaves this to autograd. */
 size_t moe_combine_add_rms_norm_bwd_ws_bytes(int64_t T, int H);
 int moe_combine_add_rms_norm_bwd(const void* dnormed, const void* dsum, const void* sum, const float* rstd, const void* gamma,
                                  const void* y, const int32_t* inv_sort_idx, const void* weights, float scale, void* dresidual,
                                  void* dy, void* dweights, void* dgamma, int64_t T, int k, int H, int dtype, void* ws,
                                  size_t ws_bytes, void* stream);
+int moe_combine_add_rms_norm_bwd_inputs(const void* dnormed, const void* dsum, const void* residual, const float* rstd,
+                                        const void* gamma, const void* y, const int32_t* inv_sort_idx, const void* weights,
+                                        float scale, void* dresidual, void* dy, void* dweights, void* dgamma, int64_t T, int k,
+                                        int H, int dtype, void* ws, size_t ws_bytes, void* stream);
 
 /* y = sum_i x_i W_i^T (which = 0, W_i (E, N, K_i)) or sum_i x_i W_i (which = 1, W_i (E, K_i, N)) per expert, the n <= 4
  * operand pairs contracted into one fp32 accumulator and rounded once.  x_i has M rows of K_i elements, ldx[i] apart.

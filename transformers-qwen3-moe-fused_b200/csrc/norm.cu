@@ -7,7 +7,11 @@
 //   dy[inv] = scale * weights * ds,   dweights[t, j] = scale <ds[t], y[inv[t k + j]]>.
 //
 // Everything between loads and stores is fp32; s and n are each rounded once (n from the sum that has not been rounded).
-// The backward pass reads s as it was stored: its rounding is that of a stored activation.
+// The backward pass forms s again from the residual and y, in the order of the forward pass and with its bits: s as it was stored
+// is off by its rounding (2.4e-3 in place of 1.7e-3 of a gradient's 2-norm in bf16), or infinite where the sum is past fp16's range
+// and n is not.  With k expert rows, which the gradient of the weights reads anyway, no more bytes are moved (residual in place of
+// s): 145 us for 139 at 8191 x 2048, k = 8; with one row (add) another T H values are: 78 for 70 at 16001 x 2048.  A caller that
+// kept s alone can give that.
 //
 // Bound by HBM.  A CTA owns a token: its k rows (k H values) are in flight at once, the row stays in registers between the
 // sum and the norm, and a decoding step of one token takes one trip to memory instead of k.  dgamma is a sum over all
@@ -20,7 +24,8 @@ namespace {
 
 constexpr int NORM_THREADS = 256;    // most threads of a CTA
 constexpr int NORM_MAX_VPT = 4;      // vectors of 16 bytes that a thread keeps of a row
-constexpr int NORM_MAX_H = 24576;    // the generic form keeps two fp32 rows in shared memory
+constexpr int NORM_MAX_H = 24576;    // the generic form keeps two fp32 rows in shared memory, or three up to
+constexpr int NORM_THREE_ROWS_H = 19200;
 constexpr int NORM_BWD_CTAS_PER_SM = 5;  // at most; the rows of partial sums are laid out for that many
 
 struct NormFwd {
@@ -40,7 +45,8 @@ struct NormFwd {
 struct NormBwd {
   const void* dnormed;
   const void* dsum;
-  const void* sum;
+  const void* base;  // the residual (may be null), or s as it was stored
+  bool stored;       // base is s
   const float* rstd;
   const void* gamma;
   const void* y;
@@ -53,6 +59,7 @@ struct NormBwd {
   float* partial;  // dgamma: one row of H sums for each CTA
   int64_t tokens;
   int k, H;
+  bool u_row;      // the generic form has room for a third fp32 row
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -223,6 +230,7 @@ norm_bwd_kernel(const NormBwd p) {
 #pragma unroll
     for (int q = 0; q < V; ++q) dg[i][q] = 0.f;
   int flip = 0, dflip = 0;
+  const bool again = p.dnormed && !p.stored;  // s is formed again
   // dweights of rows j0.. of token t from this thread's products with them
   auto store_dots = [&](float (&dot)[8], int64_t t, int j0, int nj) {
     const float v = warp_sum8(dot, lane);
@@ -237,13 +245,14 @@ norm_bwd_kernel(const NormBwd p) {
   };
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     float ds[VPT][V];  // first a, then the gradient of the sum
-    Vec<T> sv[VPT], d0[VPT];
+    float u[VPT][V];
+    Vec<T> d0[VPT];
     Vec<T> rows[FORM == BWD_COMBINE8 ? 8 : 1];
     int32_t idx[FORM == BWD_COMBINE8 ? 8 : 1];
     if constexpr (FORM == BWD_COMBINE8) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) idx[j] = p.inv[t * 8 + j];
-      if (p.dweights && (int)threadIdx.x < hv) {
+      if ((p.dweights || again) && (int)threadIdx.x < hv) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           *reinterpret_cast<uint4*>(rows[j].v) = __ldcs(reinterpret_cast<const uint4*>(y + (int64_t)idx[j] * p.H) + threadIdx.x);
@@ -259,14 +268,36 @@ norm_bwd_kernel(const NormBwd p) {
       if (!p.dnormed) continue;
       Vec<T> dn;
       *reinterpret_cast<uint4*>(dn.v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.dnormed + t * p.H) + c);
-      *reinterpret_cast<uint4*>(sv[i].v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.sum + t * p.H) + c);
+      Vec<T> b, x;
+      if (p.base) *reinterpret_cast<uint4*>(b.v) = __ldcs(reinterpret_cast<const uint4*>((const T*)p.base + t * p.H) + c);
+      if (FORM == BWD_ADD && again) *reinterpret_cast<uint4*>(x.v) = __ldcs(reinterpret_cast<const uint4*>(y + t * p.H) + c);
+      if (!again) {
+#pragma unroll
+        for (int q = 0; q < V; ++q) u[i][q] = to_f32(b.v[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < V; ++q) u[i][q] = 0.f;
+        if constexpr (FORM == BWD_ADD) {
+          add_scaled<T>(u[i], 1.f, x);
+        } else if constexpr (FORM == BWD_COMBINE8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) add_scaled<T>(u[i], to_f32(((const T*)p.weights)[t * 8 + j]), rows[j]);
+        } else {
+#pragma unroll 4
+          for (int j = 0; j < p.k; ++j)
+            add_scaled<T>(u[i], to_f32(((const T*)p.weights)[t * p.k + j]), load_vec(y + (int64_t)p.inv[t * p.k + j] * p.H + c * V));
+        }
+#pragma unroll
+        for (int q = 0; q < V; ++q) u[i][q] = p.base ? fmaf(p.scale, u[i][q], to_f32(b.v[q])) : p.scale * u[i][q];
+      }
       const Vec<T> g = load_vec((const T*)p.gamma + c * V);
 #pragma unroll
       for (int q = 0; q < V; ++q) {
-        const float d = to_f32(dn.v[q]), u = to_f32(sv[i].v[q]) * rstd;
-        dg[i][q] = fmaf(d, u, dg[i][q]);
+        const float d = to_f32(dn.v[q]);
+        u[i][q] *= rstd;
+        dg[i][q] = fmaf(d, u[i][q], dg[i][q]);
         ds[i][q] = d * to_f32(g.v[q]);
-        au = fmaf(ds[i][q], u, au);
+        au = fmaf(ds[i][q], u[i][q], au);
       }
     }
     if (p.dnormed) {
@@ -281,7 +312,7 @@ norm_bwd_kernel(const NormBwd p) {
 #pragma unroll
       for (int q = 0; q < V; ++q) {
         float v = p.dsum ? to_f32(d0[i].v[q]) : 0.f;
-        if (p.dnormed) v = fmaf(rstd, ds[i][q] - to_f32(sv[i].v[q]) * rstd * au, v);
+        if (p.dnormed) v = fmaf(rstd, ds[i][q] - u[i][q] * au, v);
         ds[i][q] = v;
         o.v[q] = from_f32<T>(v);
         ox.v[q] = from_f32<T>(p.scale * v);
@@ -358,23 +389,42 @@ norm_bwd_kernel(const NormBwd p) {
   }
 }
 
-template <typename T>
+// (The form of the sum as a parameter: with tests of it between the loads of a column, add took 102 us
+// at 8191 x 1001, for 72.)
+enum NormBwdSum { SUM_STORED, SUM_ADD, SUM_COMBINE };
+template <typename T, int SUM>
 __global__ void __launch_bounds__(NORM_THREADS)
 norm_bwd_generic_kernel(const NormBwd p) {
   extern __shared__ float rows[];
   float* ds = rows;
   float* dg = rows + p.H;
+  float* us = p.u_row ? rows + 2 * p.H : nullptr;  // (the longest rows: formed twice)
   __shared__ float red[2][NORM_THREADS / 32];
   const T* y = (const T*)p.y;
-  // (a thread reads and writes its own columns of both rows only)
+  auto sum_at = [&](int64_t t, int c) {
+    const float b = p.base ? to_f32(((const T*)p.base)[t * p.H + c]) : 0.f;
+    if constexpr (SUM == SUM_STORED) return b;
+    float s = 0.f;
+    if constexpr (SUM == SUM_COMBINE) {
+#pragma unroll 4
+      for (int j = 0; j < p.k; ++j)
+        s = fmaf(to_f32(((const T*)p.weights)[t * p.k + j]), to_f32(y[(int64_t)p.inv[t * p.k + j] * p.H + c]), s);
+    } else {
+      s = to_f32(y[t * p.H + c]);
+    }
+    return p.base ? fmaf(p.scale, s, b) : p.scale * s;
+  };
+  // (a thread reads and writes its own columns of the rows only)
   for (int c = threadIdx.x; c < p.H; c += NORM_THREADS) dg[c] = 0.f;
   int flip = 0;
   for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
     const float rstd = p.dnormed ? p.rstd[t] : 0.f;
     float au = 0.f;
     if (p.dnormed) {
+#pragma unroll 4
       for (int c = threadIdx.x; c < p.H; c += NORM_THREADS) {
-        const float d = to_f32(((const T*)p.dnormed)[t * p.H + c]), u = to_f32(((const T*)p.sum)[t * p.H + c]) * rstd;
+        const float d = to_f32(((const T*)p.dnormed)[t * p.H + c]), u = sum_at(t, c) * rstd;
+        if (us) us[c] = u;
         const float a = d * to_f32(((const T*)p.gamma)[c]);
         dg[c] = fmaf(d, u, dg[c]);
         ds[c] = a;
@@ -385,7 +435,7 @@ norm_bwd_generic_kernel(const NormBwd p) {
     }
     for (int c = threadIdx.x; c < p.H; c += NORM_THREADS) {
       float v = p.dsum ? to_f32(((const T*)p.dsum)[t * p.H + c]) : 0.f;
-      if (p.dnormed) v = fmaf(rstd, ds[c] - to_f32(((const T*)p.sum)[t * p.H + c]) * rstd * au, v);
+      if (p.dnormed) v = fmaf(rstd, ds[c] - (us ? us[c] : sum_at(t, c) * rstd) * au, v);
       ds[c] = v;
       if (p.dresidual) ((T*)p.dresidual)[t * p.H + c] = from_f32<T>(v);
       if (!p.inv && p.dy) ((T*)p.dy)[t * p.H + c] = from_f32<T>(p.scale * v);
@@ -464,7 +514,7 @@ int launch_fwd(const NormFwd& p, bool vec, cudaStream_t stream) {
 }
 
 template <typename T>
-int launch_bwd(const NormBwd& p, void* dgamma, bool vec, cudaStream_t stream) {
+int launch_bwd(NormBwd& p, void* dgamma, bool vec, cudaStream_t stream) {
   const RowShape rs = vec ? row_shape(p.H / Vec<T>::N) : RowShape{0, 0};
   int grid = bwd_grid(p.tokens);
   // as many CTAs as are resident at once: each walks several tokens and leaves one row of partial sums
@@ -485,12 +535,14 @@ int launch_bwd(const NormBwd& p, void* dgamma, bool vec, cudaStream_t stream) {
     MOE_NORM_BWD(4, BWD_COMBINE)
 #undef MOE_NORM_BWD
   } else {
-    const int smem = 2 * p.H * (int)sizeof(float);
+    p.u_row = !p.stored && p.H <= NORM_THREE_ROWS_H;
+    const int smem = (p.u_row ? 3 : 2) * p.H * (int)sizeof(float);
+    auto* kernel = p.stored ? norm_bwd_generic_kernel<T, SUM_STORED> : p.inv ? norm_bwd_generic_kernel<T, SUM_COMBINE> : norm_bwd_generic_kernel<T, SUM_ADD>;
     if (smem > 48 * 1024) {
-      const int st = cuda_status(cudaFuncSetAttribute(norm_bwd_generic_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      const int st = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
       if (st != MOE_OK) return st;
     }
-    norm_bwd_generic_kernel<T><<<grid, NORM_THREADS, smem, stream>>>(p);
+    kernel<<<grid, NORM_THREADS, smem, stream>>>(p);
   }
   int st = launch_status();
   if (st != MOE_OK || !p.partial) return st;
@@ -527,10 +579,9 @@ MOE_API size_t moe_combine_add_rms_norm_bwd_ws_bytes(int64_t T_, int H) {
   return (size_t)bwd_grid(T_) * H * sizeof(float);
 }
 
-MOE_API int moe_combine_add_rms_norm_bwd(const void* dnormed, const void* dsum, const void* sum, const float* rstd,
-                                         const void* gamma, const void* y, const int32_t* inv_sort_idx, const void* weights,
-                                         float scale, void* dresidual, void* dy, void* dweights, void* dgamma, int64_t T_, int k,
-                                         int H, int dtype, void* ws, size_t ws_bytes, void* stream) {
+static int norm_bwd(const void* dnormed, const void* dsum, const void* base, bool stored, const float* rstd, const void* gamma,
+                    const void* y, const int32_t* inv_sort_idx, const void* weights, float scale, void* dresidual, void* dy,
+                    void* dweights, void* dgamma, int64_t T_, int k, int H, int dtype, void* ws, size_t ws_bytes, void* stream) {
   if (!is_float_dtype(dtype)) return MOE_ERR_DTYPE;
   if (!norm_extents_ok(T_, k, H, inv_sort_idx != nullptr)) return MOE_ERR_SHAPE;
   if (dgamma && (T_ == 0 || !dnormed)) {
@@ -539,14 +590,31 @@ MOE_API int moe_combine_add_rms_norm_bwd(const void* dnormed, const void* dsum, 
     dgamma = nullptr;
   }
   if (T_ == 0 || (!dresidual && !dy && !dweights && !dgamma)) return MOE_OK;
-  if (dnormed && (!sum || !rstd || !gamma)) return MOE_ERR_NULL;
+  if (dnormed && (!rstd || !gamma || (stored ? !base : !y || (inv_sort_idx && !weights)))) return MOE_ERR_NULL;
   if (inv_sort_idx ? (dy && !weights) || (dweights && !y) : dweights != nullptr) return MOE_ERR_NULL;
   if (dgamma && (!ws || ((uintptr_t)ws & 15) || ws_bytes < moe_combine_add_rms_norm_bwd_ws_bytes(T_, H))) return MOE_ERR_WORKSPACE;
-  const NormBwd p{dnormed, dsum, sum, rstd, gamma, y, inv_sort_idx, weights, scale, dresidual, dy, dweights,
-                  dgamma ? (float*)ws : nullptr, T_, k, H};
+  NormBwd p{dnormed, dsum, base, stored, rstd, gamma, y, inv_sort_idx, weights, scale, dresidual, dy, dweights,
+            dgamma ? (float*)ws : nullptr, T_, k, H, false};
   MOE_DISPATCH_FLOAT(dtype, T, {
-    const bool vec = H % Vec<T>::N == 0 && aligned16(dnormed) && aligned16(dsum) && aligned16(sum) && aligned16(gamma) &&
+    const bool vec = H % Vec<T>::N == 0 && aligned16(dnormed) && aligned16(dsum) && aligned16(base) && aligned16(gamma) &&
                      aligned16(y) && aligned16(dresidual) && aligned16(dy);
     return launch_bwd<T>(p, dgamma, vec, (cudaStream_t)stream);
   });
+}
+
+MOE_API int moe_combine_add_rms_norm_bwd(const void* dnormed, const void* dsum, const void* sum, const float* rstd,
+                                         const void* gamma, const void* y, const int32_t* inv_sort_idx, const void* weights,
+                                         float scale, void* dresidual, void* dy, void* dweights, void* dgamma, int64_t T_, int k,
+                                         int H, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  return norm_bwd(dnormed, dsum, sum, true, rstd, gamma, y, inv_sort_idx, weights, scale, dresidual, dy, dweights, dgamma, T_, k, H,
+                  dtype, ws, ws_bytes, stream);
+}
+
+MOE_API int moe_combine_add_rms_norm_bwd_inputs(const void* dnormed, const void* dsum, const void* residual, const float* rstd,
+                                                const void* gamma, const void* y, const int32_t* inv_sort_idx,
+                                                const void* weights, float scale, void* dresidual, void* dy, void* dweights,
+                                                void* dgamma, int64_t T_, int k, int H, int dtype, void* ws, size_t ws_bytes,
+                                                void* stream) {
+  return norm_bwd(dnormed, dsum, residual, false, rstd, gamma, y, inv_sort_idx, weights, scale, dresidual, dy, dweights, dgamma, T_,
+                  k, H, dtype, ws, ws_bytes, stream);
 }

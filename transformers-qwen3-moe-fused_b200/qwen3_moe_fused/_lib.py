@@ -66,6 +66,7 @@ SIGNATURES = {
     "moe_combine_add_rms_norm": (_I, [_P, _P, _P, _P, _P, _F, _F, _P, _P, _P, _L, _I, _I, _I, _P]),
     "moe_combine_add_rms_norm_bwd_ws_bytes": (_Z, [_L, _I]),
     "moe_combine_add_rms_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _L, _I, _I, _I, _P, _Z, _P]),
+    "moe_combine_add_rms_norm_bwd_inputs": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _L, _I, _I, _I, _P, _Z, _P]),
     "moe_block_fwd_scratch_bytes": (_Z, [_L, _I, _I, _I, _I, _I]),
     "moe_block_fwd": (_I, [_P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _P, _Z, _P]),
     "moe_lora_mlp_fwd": (_I, [_P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _P]),

@@ -33,49 +33,49 @@ class CombineAddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, inv_sort_idx, weights, residual, gamma, eps, scale):
         normed, total, rstd = _forward(y, inv_sort_idx, weights, residual, gamma, eps, scale, True)
-        # y is read again for the routing weights' gradient only
-        keep_y = weights is not None and ctx.needs_input_grad[2]
-        ctx.save_for_backward(y if keep_y else None, inv_sort_idx, weights, gamma, total, rstd)
-        ctx.scale, ctx.y_shape = scale, y.shape
+        # the backward forms the sum again: `total` has been rounded, and may be infinite in fp16 where `normed` is not
+        ctx.save_for_backward(y, inv_sort_idx, weights, residual, gamma, rstd)
+        ctx.scale, ctx.y_shape, ctx.k = scale, y.shape, 1 if weights is None else weights.shape[1]
         ctx.set_materialize_grads(False)
         return normed, total
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dnormed, dtotal):
-        y, inv_sort_idx, weights, gamma, total, rstd = ctx.saved_tensors
-        T, H = total.shape
-        k = 1 if weights is None else weights.shape[1]
+        y, inv_sort_idx, weights, residual, gamma, rstd = ctx.saved_tensors
+        rows, H = ctx.y_shape
+        T, k = rstd.shape[0], ctx.k
         want_y, _, want_w, want_r, want_g = ctx.needs_input_grad[:5]
         if dnormed is None and dtotal is None:
             return (None,) * 7
+        some = dtotal if dnormed is None else dnormed
 
         # (hooks on saved tensors may have given back another type, device or layout)
-        def like_total(t, shape, dtype=total.dtype):
-            if t is not None and (t.shape != shape or t.dtype != dtype or t.device != total.device or not t.is_contiguous()):
+        def checked(t, shape, dtype=some.dtype):
+            if t is not None and (t.shape != shape or t.dtype != dtype or t.device != some.device or not t.is_contiguous()):
                 raise _lib.MoeB200Error("combine_add_rms_norm: a tensor of the backward pass has another type, device or layout "
                                         "than in the forward pass")
             return t
 
-        dnormed = None if dnormed is None else like_total(dnormed.contiguous(), (T, H))
-        dtotal = None if dtotal is None else like_total(dtotal.contiguous(), (T, H))
-        like_total(total, (T, H)), like_total(rstd, (T,), torch.float32), like_total(gamma, (H,)), like_total(y, ctx.y_shape)
-        like_total(weights, (T, k)), like_total(inv_sort_idx, (T * k,), torch.int32)
+        dnormed = None if dnormed is None else checked(dnormed.contiguous(), (T, H))
+        dtotal = None if dtotal is None else checked(dtotal.contiguous(), (T, H))
+        checked(residual, (T, H)), checked(rstd, (T,), torch.float32), checked(gamma, (H,)), checked(y, (rows, H))
+        checked(weights, (T, k)), checked(inv_sort_idx, (rows,), torch.int32)
 
         def out(want, *shape):
-            return torch.empty(shape, device=total.device, dtype=total.dtype) if want else None
+            return torch.empty(shape, device=some.device, dtype=some.dtype) if want else None
 
-        dy, dw, dr, dg = out(want_y, *ctx.y_shape), out(want_w, T, k), out(want_r, T, H), out(want_g, H)
+        dy, dw, dr, dg = out(want_y, rows, H), out(want_w, T, k), out(want_r, T, H), out(want_g, H)
         lib = _lib.load()
         nbytes = lib.moe_combine_add_rms_norm_bwd_ws_bytes(T, H) if want_g else 0
-        here, stream = _lib.launch_on(total.device)
+        here, stream = _lib.launch_on(some.device)
         with here:
-            ws = torch.empty(nbytes, device=total.device, dtype=torch.uint8) if nbytes else None
-            status = lib.moe_combine_add_rms_norm_bwd(
-                _lib.ptr(dnormed), _lib.ptr(dtotal), _lib.ptr(total), _lib.ptr(rstd), _lib.ptr(gamma), _lib.ptr(y),
+            ws = torch.empty(nbytes, device=some.device, dtype=torch.uint8) if nbytes else None
+            status = lib.moe_combine_add_rms_norm_bwd_inputs(
+                _lib.ptr(dnormed), _lib.ptr(dtotal), _lib.ptr(residual), _lib.ptr(rstd), _lib.ptr(gamma), _lib.ptr(y),
                 _lib.ptr(inv_sort_idx), _lib.ptr(weights), ctx.scale, _lib.ptr(dr), _lib.ptr(dy), _lib.ptr(dw), _lib.ptr(dg),
-                T, k, H, _lib.float_code(total.dtype), _lib.ptr(ws), nbytes, stream)
-        _lib.check(status, "moe_combine_add_rms_norm_bwd")
+                T, k, H, _lib.float_code(some.dtype), _lib.ptr(ws), nbytes, stream)
+        _lib.check(status, "moe_combine_add_rms_norm_bwd_inputs")
         return dy, None, dw, dr, dg, None, None
 
 
@@ -100,7 +100,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torc
                  scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """(normed, sum) with sum = residual + scale * x and normed = sum / sqrt(mean(sum^2) + eps) * weight over the last
     dimension (1 to 24576); `residual` None: zeros.  Both shaped like x.  x, residual and weight have one floating type; the
-    arithmetic is fp32 and each output is rounded once.  Gradients for all three, once (no second derivative)."""
+    arithmetic is fp32 and each output is rounded once.  Gradients for all three, once (no second derivative); x and residual are kept
+    for them."""
     assert x.ndim >= 1 and x.shape[-1] >= 1
     H = x.shape[-1]
     rows = x.numel() // H
@@ -115,7 +116,7 @@ def combine_add_rms_norm(y: torch.Tensor, sort_idx: torch.Tensor, inv_sort_idx: 
     """`add_rms_norm` on the block's combined output, which is not written: with `routing_weights` (T, k) and the expert
     rows y (T * k, H) in sorted order, sum[t] = residual[t] + scale * sum_j routing_weights[t, j] * y[inv_sort_idx[t*k + j]].
     `sort_idx`, `inv_sort_idx`: as for `combine`, int32, each row once.  `residual`: T * H values; the outputs are shaped like it,
-    (T, H) without one.  Gradients for y, routing_weights, residual and weight, once."""
+    (T, H) without one.  Gradients for y, routing_weights, residual and weight, once; all of them are kept for that."""
     assert y.ndim == 2 and routing_weights.ndim == 2 and y.shape[1] >= 1
     T, k = routing_weights.shape
     H = y.shape[1]
