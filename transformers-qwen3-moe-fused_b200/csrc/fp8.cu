@@ -145,7 +145,7 @@ silu_quantize_kernel(const float* __restrict__ e, const float* __restrict__ g, i
       float h[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        h[i] = gated_silu(v.e.v[i], v.g.v[i]);
+        h[i] = gated_silu<T>(v.e.v[i], v.g.v[i]);
         if (keep_e && at.col + i < I) {
           keep_e[at.row * I + at.col + i] = from_f32<T>(v.e.v[i]);
           keep_g[at.row * I + at.col + i] = from_f32<T>(v.g.v[i]);
@@ -171,7 +171,7 @@ silu_bwd_quantize_kernel(const float* __restrict__ dh, const T* __restrict__ e, 
     [&](const RowBlock& at, const Values& v) {
       float de[8], dg[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) gated_silu_bwd(v.dh.v[i], to_f32(v.e.v[i]), to_f32(v.g.v[i]), de[i], dg[i]);
+      for (int i = 0; i < 8; ++i) gated_silu_bwd<T>(v.dh.v[i], to_f32(v.e.v[i]), to_f32(v.g.v[i]), de[i], dg[i]);
       store_codes<VEC>(de, top_of(de), deq + at.row * I, at.col, I, des + at.kb * pitch + at.row);
       store_codes<VEC>(dg, top_of(dg), dgq + at.row * I, at.col, I, dgs + at.kb * pitch + at.row);
     });

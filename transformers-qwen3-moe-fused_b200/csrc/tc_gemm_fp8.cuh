@@ -473,7 +473,8 @@ pair_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {  // (features past the last one have zeros in both)
-          const float h0 = gated_silu(lo_f32(acc[i]), lo_f32(acc[32 + i])), h1 = gated_silu(hi_f32(acc[i]), hi_f32(acc[32 + i]));
+          const float h0 = gated_silu<__half>(lo_f32(acc[i]), lo_f32(acc[32 + i]));  // (either 16-bit type)
+          const float h1 = gated_silu<__half>(hi_f32(acc[i]), hi_f32(acc[32 + i]));
           top = max(top, max(magnitude_bits(h0), magnitude_bits(h1)));
           acc[i] = pack_f32x2(__float_as_uint(h0), __float_as_uint(h1));
         }

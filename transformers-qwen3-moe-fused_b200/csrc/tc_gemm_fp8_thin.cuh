@@ -293,7 +293,7 @@ thin_fp8_kernel(const __grid_constant__ Fp8Maps maps, const Fp8Params p) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           if (i < rows) {  // (features past the last one have zeros in both)
-            acc[0][i] = gated_silu(acc[0][i], acc[WEIGHTS - 1][i]);
+            acc[0][i] = gated_silu<__half>(acc[0][i], acc[WEIGHTS - 1][i]);  // (either 16-bit type)
             const uint32_t top = __reduce_max_sync(0xffffffffu, magnitude_bits(acc[0][i]));
             if (lane == 0) ctl->tops[i][quarter] = top;
           }
