@@ -205,7 +205,7 @@ int moe_nf4_dequant(const uint8_t* packed, const float* code, const float* absma
  * (qwen3_moe_fused/grouped_gemm/forward_4bit.py).
  * Weights: e4m3 codes w (E,N,K) and fp32 scales ws (E, ceil(N/128), ceil(K/128)); a weight is code * scale of its block.
  * Activations: e4m3 codes q (M,K) and fp32 scales s (ceil(K/128), M): block-major, M rounded up to a multiple of 4 elements
- * from one block to the next (what lies between is not read or written), one power of two for each 128 values of a row,
+ * from one block to the next (what lies between is not read or written), of any 4-byte alignment, one power of two for each 128 values of a row,
  * the smallest with max|x| <= 448 s (at least 2^-100), NaN for a block that holds an infinity or a NaN.  Codes are rounded
  * to nearest, ties to even.
  * ------------------------------------------------------------------------------- */

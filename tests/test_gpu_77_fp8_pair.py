@@ -18,6 +18,37 @@ def pairs():
     assert _lib.read_error_flag() == 0
 
 
+@pytest.mark.parametrize("path", ["PATH_TC", "PATH_TC_SINGLE"])
+def test_scales_of_any_alignment(cuda, path):
+    """Scales that start between two 16-byte units: the tensor-core kernels take them, with the same bits."""
+    from qwen3_moe_fused import _lib
+    from qwen3_moe_fused.quantize.fp8 import quantize_fp8_rows
+
+    gen = products.gen_for(cuda, 21)
+    M, K, N, E = 200, 384, 256, 2
+    codes, ws = products.fp8_weight(E, N, K, gen, cuda)
+    q, s = quantize_fp8_rows(torch.randn(M, K, generator=gen, device=cuda).to(torch.bfloat16))
+    m_sizes = torch.tensor([130, 70], device=cuda, dtype=torch.int32)
+    y = torch.empty(M, N, device=cuda, dtype=torch.bfloat16)
+    prev = _lib.set_gemm_path(getattr(_lib, path))
+    try:
+        got = []
+        for offset in (0, 1, 2, 3):
+            base = torch.empty(s.shape[0] * s.stride(0) + offset, device=cuda)[offset:]
+            scales = base.as_strided(s.shape, s.stride())
+            scales.copy_(s)
+            st = _lib.load().moe_grouped_gemm_fp8(0, q.data_ptr(), scales.data_ptr(), codes.data_ptr(), ws.data_ptr(), None, None, None,
+                                                  None, m_sizes.data_ptr(), _lib.I32, y.data_ptr(), M, N, K, E, _lib.BF16,
+                                                  _lib.stream_ptr(cuda))
+            _lib.check(st, "moe_grouped_gemm_fp8")
+            got.append(y.clone())
+        assert all(torch.equal(g, got[0]) for g in got)
+        torch.cuda.synchronize()
+        assert _lib.read_error_flag() == 0
+    finally:
+        _lib.set_gemm_path(prev)
+
+
 @pytest.mark.parametrize("K,N", [(2048, 1536), (128, 512), (384, 208)])
 def test_the_same_bits_in_every_run(cuda, pairs, K, N):
     """Accumulators are handed back and overwritten a few hundred cycles after they are read: a reading that came late would show."""

@@ -56,7 +56,8 @@ inline int sm_count() {
   return cached[dev];
 }
 
-// Elements between the blocks of the scales of M quantised rows: whole 16-byte units, as the copy engine wants them.
+// Elements between the blocks of the scales of M quantised rows: whole 16-byte units.  (Part of the layout; the kernels read and
+// write scales one at a time and need no more than their own alignment.)
 __host__ __device__ inline int64_t fp8_scale_pitch(int64_t M) { return (M + 3) & ~(int64_t)3; }
 
 // moe_grouped_gemm_sum whose product i counts 2^log2_scale[i] times (null: once; at most 2^15 between any two), and

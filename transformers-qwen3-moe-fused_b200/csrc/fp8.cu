@@ -11,8 +11,7 @@
 
 namespace moe {
 
-bool tc_fp8_eligible(const void* q, const float* s, const void* w, const void* q2, const float* s2, const void* w2, const void* out,
-                     int64_t M, int N, int K, int E);
+bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E);
 int tc_grouped_gemm_fp8(int which, const void* q, const float* s, const void* w, const float* ws, const void* q2, const float* s2,
                         const void* w2, const float* ws2, const void* m_sizes, int ms64, void* out, int64_t M, int N, int K, int E,
                         int dtype_out, int form, cudaStream_t stream);
@@ -350,7 +349,7 @@ MOE_API int moe_gate_up_silu_fp8(const void* q, const float* s, const void* w_ga
   if (!q || !s || !w_gate || !ws_gate || !w_up || !ws_up || !m_sizes || !hq || !hs || !keep_e != !keep_g) return MOE_ERR_NULL;
   const int path = moe_get_gemm_path();
   if (path == MOE_PATH_SIMT || dtype == MOE_F32 || !aligned16(keep_e) || !aligned16(keep_g) ||
-      !tc_fp8_eligible(q, s, w_gate, nullptr, nullptr, w_up, hq, M, I, K, E))
+      !tc_fp8_eligible(q, w_gate, nullptr, w_up, hq, M, I, K, E))
     return MOE_ERR_UNSUPPORTED;
   return tc_gate_up_silu_fp8(q, s, w_gate, ws_gate, w_up, ws_up, m_sizes, msd == MOE_I64, hq, hs, keep_e, keep_g, M, I, K, E, dtype,
                              path, (cudaStream_t)stream);
@@ -366,7 +365,7 @@ MOE_API int moe_grouped_gemm_fp8(int which, const void* q, const float* s, const
   if (!q || !s || !w || !ws || !m_sizes || !y || (q2 && (!s2 || !w2 || !ws2))) return MOE_ERR_NULL;
   const int ms64 = msd == MOE_I64;
   const int path = moe_get_gemm_path();
-  if (path != MOE_PATH_SIMT && tc_fp8_eligible(q, s, w, q2, s2, w2, y, M, N, K, E))
+  if (path != MOE_PATH_SIMT && tc_fp8_eligible(q, w, q2, w2, y, M, N, K, E))
     return tc_grouped_gemm_fp8(which, q, s, w, ws, q2, s2, w2, ws2, m_sizes, ms64, y, M, N, K, E, dtype_out, path, stream);
   if (path == MOE_PATH_TC || path == MOE_PATH_TC_SINGLE) return MOE_ERR_UNSUPPORTED;
   const Fp8Pairs ops = {{(const uint8_t*)q, (const uint8_t*)q2}, {s, s2}, {(const uint8_t*)w, (const uint8_t*)w2}, {ws, ws2}, q2 ? 2 : 1};

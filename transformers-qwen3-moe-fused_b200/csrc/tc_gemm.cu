@@ -1244,10 +1244,10 @@ int tc_grouped_gemm_nf4(const void* x, const uint8_t* packed, const float* code,
   return launch_status();
 }
 
-// What the 8-bit CTA-pair kernel takes: rows of 16-byte multiples on aligned bases, tables of the groups in shared memory.
-bool tc_fp8_eligible(const void* q, const float* s, const void* w, const void* q2, const float* s2, const void* w2, const void* out,
-                     int64_t M, int N, int K, int E) {
-  const uintptr_t bits = (uintptr_t)q | (uintptr_t)w | (uintptr_t)q2 | (uintptr_t)w2 | (uintptr_t)out | (uintptr_t)s | (uintptr_t)s2;
+// What the 8-bit tensor-core kernels take: rows of 16-byte multiples on aligned bases (scales are read one at a time), tables of the
+// groups in shared memory.
+bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w2, const void* out, int64_t M, int N, int K, int E) {
+  const uintptr_t bits = (uintptr_t)q | (uintptr_t)w | (uintptr_t)q2 | (uintptr_t)w2 | (uintptr_t)out;
   if ((bits & 15) || N % 16 || K % 16 || E > tc::MAX_E || M < 1 || M > 0x7fffffffLL - 1024) return false;
   return pair_tiles_bound(M, E, (N + 255) / 256) < (int64_t)1 << 30;  // tile ids and grids are 32-bit
 }
