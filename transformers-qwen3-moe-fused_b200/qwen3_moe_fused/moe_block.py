@@ -14,7 +14,6 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd import forward_ad
 
 from . import _lib
 from .functional import moe_fused_linear
@@ -65,12 +64,6 @@ def route(router_logits: torch.Tensor, num_selected: int, norm_topk_prob: bool, 
     return softmax_topk_autograd(router_logits.contiguous(), num_selected, norm_topk_prob, dtype)
 
 
-def _has_tangent(*tensors) -> bool:
-    """Whether a tensor carries a forward-mode derivative.  Grad mode does not switch forward mode off, and a call that
-    takes addresses would lose the tangent without a word: such tensors go through the autograd functions, which raise."""
-    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
-
-
 def _block_infer(x, router_logits, gate_proj, up_proj, down_proj, k: int, norm_topk_prob: bool) -> Optional[torch.Tensor]:
     """The block after its router GEMM as one call into the library (the same kernels in the same order as the
     composition in `moe_block_forward`); None where that composition has to decide: other dtypes, layouts, extents."""
@@ -111,7 +104,7 @@ def moe_block_forward(hidden_states: torch.Tensor, gate_weight: torch.Tensor, ga
     k = num_selected
     x = hidden_states.reshape(T, H)
     router_logits = torch.nn.functional.linear(x, gate_weight)
-    infer = not torch.is_grad_enabled() and not _has_tangent(x, router_logits, gate_proj, up_proj, down_proj)
+    infer = not torch.is_grad_enabled() and not _lib.has_tangent(x, router_logits, gate_proj, up_proj, down_proj)
     if infer and not GATHER_IN_KERNEL:
         out = _block_infer(x, router_logits, gate_proj, up_proj, down_proj, k, norm_topk_prob)
         if out is not None:
@@ -162,7 +155,7 @@ def moe_layer_forward(hidden_states: torch.Tensor, residual: Optional[torch.Tens
         y = moe_mlp_fp8(rows, *projections, m_sizes)
     else:
         gate_proj, up_proj, down_proj = projections
-        infer = not torch.is_grad_enabled() and not _has_tangent(rows, gate_proj, up_proj, down_proj)
+        infer = not torch.is_grad_enabled() and not _lib.has_tangent(rows, gate_proj, up_proj, down_proj)
         y = moe_fused_linear((gate_up_silu_forward if infer else gate_up_silu)(rows, gate_proj, up_proj, m_sizes), down_proj, m_sizes)
     normed, out = combine_add_rms_norm(y, sort_idx, inv_sort_idx, routing_weights, stream, next_norm_weight, eps, scale)
     return normed, out, router_logits
