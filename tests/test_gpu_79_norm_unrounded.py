@@ -37,7 +37,8 @@ def check(grads, x, scale, dtype, inv=None):
 
 
 # one vector of a row to a thread, two, four; rows in shared memory, three of them and two
-SHAPES = [(301, 2048, 8), (33, 1024, 4), (70, 4096, 8), (9, 8192, 3), (40, 1001, 5), (5, 8200, 9), (2, 24576, 2), (3, 24575, 1), (6, 1, 2)]
+SHAPES = [(301, 2048, 8), (33, 1024, 4), (70, 4096, 8), (9, 8192, 3), (40, 1001, 5), (5, 8200, 9), (2, 19200, 2), (2, 19201, 3), (2, 24576, 2),
+          (3, 24575, 1), (6, 1, 2)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])

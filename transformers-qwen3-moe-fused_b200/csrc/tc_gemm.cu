@@ -1252,8 +1252,11 @@ bool tc_fp8_eligible(const void* q, const void* w, const void* q2, const void* w
   return pair_tiles_bound(M, E, (N + 255) / 256) < (int64_t)1 << 30;  // tile ids and grids are 32-bit
 }
 
-// Which of the two kernels: thin_fp8_kernel while the groups have few rows on average.  128 experts, 2048 -> 1536, 8192 / 12288
-// rows: 114 / 144 us against 144 / 144 of the pair kernel; gate and up of 768 features, 4096 / 6144 rows: 119 / 142 against 136 / 137.
+// Which of the two kernels: thin_fp8_kernel while the groups have few rows on average (M / E, empty groups counted).  128 experts,
+// thin / pair, us, L2 flushed.  2048 -> 1536, evenly routed: 4096 rows 94 / 139, 8192 113 / 143, 9216 131 / 141, 10240 143 / 142;
+// Zipf with empty groups: 8192 123 / 148, 10240 133 / 149, 12288 141 / 156.  768 -> 2048: 8192 80 / 90, 9216 91 / 90; Zipf 82 / 96,
+// 86 / 96.  Gate and up of 768 features: 4096 rows 115 / 130, 5120 134 / 132; Zipf 114 / 128, 126 / 130, 6144 140 / 132.  Both means
+// are a little below the crossing of even routing (72 to 80 and 40), skewed routing crosses later.
 static constexpr int64_t THIN_FP8_MEAN = 64, THIN_FP8_MEAN_GATE_UP = 32;
 static int64_t thin_tiles_bound(int64_t M, int E, int N) { return (M / 32 + (M < E ? M : E)) * ((N + 127) / 128); }  // (32: the lower tile)
 static bool thin_fp8(int form, int64_t M, int E, int N, int64_t mean) {

@@ -12,13 +12,15 @@
 // columns alternate, so the addition of one block runs beside the MMAs of the next.
 // (With weight rows as accumulator rows the factor changes from column to column.  In the fragment shape 16x256b, where a thread
 // needs few of them, TMEM loads run at half the rate: 535 cycles for 256 columns against 260 in the shape 32x32b.  Forward /
-// dX at 65536 rows, 2048 -> 1536: 401 / 424 us, against 309 / 318 us here.)
+// dX at 65536 rows, 2048 -> 1536: 401 / 424 us, against 305 / 315 us here.)
 //
-// What bounds it: the additions, not the MMAs.  With the additions left out a block takes 515 cycles, what the MMAs need at the
-// 8-bit peak, and the launch 220 us; with them 1100.  They are 256 cycles of TMEM loads and 285 of FMAs on each quarter of the
-// SM, but 128 sums, 32 loaded values and the addresses leave the compiler no registers to overlap the two (half the sums:
-// 240 us).  Narrower tiles (192 columns, 96 or 64 sums), 16 warps, four accumulators of 128 columns, scales that come by TMA, and
-// loads of 64 columns were no faster: 310 to 390 us.
+// What bounds it: the latency of the additions, not the MMAs and no throughput.  A block takes 1250 cycles (65536 rows in even
+// groups: 255 us, tensor pipe 41 %), where the MMAs need 512 (with the additions left out it takes 515), the TMEM loads 256 and
+// the FMAs 285 on each quarter of the SM, which would be 541 even one after the other.  A quarter's two warps each load 32
+// columns, wait, and issue 16 packed FMAs, four times in a row: no warp can issue in 60 % of the cycles, the fp32 pipe is 31 % busy.
+// With 128 sums and 32 loaded values a thread has no registers left for loads that run ahead (half the sums: 240 us).  Narrower
+// tiles (192 columns, 96 or 64 sums), 16 warps, four accumulators of 128 columns, scales that come by TMA, and loads of 64 columns
+// were no faster: 310 to 390 us.
 //
 // The price of tokens as rows is that a tile costs 256 rows of MMAs whatever it holds (warps without rows skip the additions);
 // groups of few rows have a kernel of their own, thin_fp8_kernel.

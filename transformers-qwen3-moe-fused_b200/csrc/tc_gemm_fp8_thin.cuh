@@ -9,8 +9,8 @@
 // i and 32 + i, four blocks ahead, and shuffles hand them round.
 // Two CTAs on an SM, 64 KB of weights under way in each, take the tiles in turn; the loads of the next tile are issued while the
 // last blocks of one are added and stored (with a CTA to a tile: 97 us for 88).
-// 384 rows, 128 experts, 2048 -> 1536: 88 us, 4.4 TB/s of weights, 84 for the gradient (pair_fp8_kernel: 121, 128); gate and up of
-// 768 features 91 (129), with 64 tokens to a tile 127; 768 -> 2048 53 (81).
+// 384 rows, 128 experts, 2048 -> 1536, L2 flushed: 82 to 88 us from box to box, 4.4 to 4.7 TB/s of weights, 82 for the gradient
+// (pair_fp8_kernel: 121, 128); gate and up of 768 features 86 (129), with 64 tokens to a tile 127; 768 -> 2048 51 (81).
 // (A counter of stages that wraps round by a comparison, in place of the low bits of a running one, cost the thread that issues
 // the MMAs 12 us of 93 at 4096 rows.)
 #pragma once
